@@ -218,6 +218,27 @@ int ppv_weight_layout(const float* w, void* out, int Cout, int Cin, int R, int S
 int ppv_adam_multi(const void* desc, int ndesc, int total_blocks, double lr, double beta1, double beta2, double eps, double weight_decay,
                    double bias_correction1, double bias_correction2, ppv_stream_t stream);
 
+/* One AdamW step (torch.optim.AdamW semantics, amsgrad = maximize = False) of a whole list of f32 tensors in one launch (csrc/adamw.hip),
+ * moments in 32 or in 8 bits.  desc: DEVICE array of ndesc 64-byte records
+ *   {float* p; const float* g; void* m; void* v; float* ms; float* vs; long numel; int blk0; unsigned stream}
+ * ms == NULL: m, v are the f32 moments.  Otherwise m and v hold OCP e4m3 codes of the first moment and of the ROOT of the second, ms and vs
+ * one f32 power-of-two scale per 256 consecutive elements of the tensor (ceil(numel / 256) each); `stream` tells the tensors apart in the
+ * random numbers of the stochastic rounding.  blk0 = prefix sum of ceil(numel / 4096) over the records, total_blocks = that sum.
+ * step counts from 1 and includes this step; seed starts the random numbers.  Tensors need the alignment of their elements only. */
+int ppv_adamw_multi(const void* desc, int ndesc, int total_blocks, double lr, double beta1, double beta2, double eps, double weight_decay,
+                    double step, unsigned seed, ppv_stream_t stream);
+
+/* ---- layer norm over the last axis (csrc/layernorm.hip) -------------------------------------------
+ * x [rows][C] with a row stride of ldx elements, y [rows][C] packed; w, b [C] or NULL (1 and 0).  dtype of x, y, g, dx and wdtype of w, b,
+ * dw, db: 0 f32, 1 bf16, 2 f16; all sums f32.  mean, rstd [rows] f32: both or neither (not wanted: no backward).  Any C, any alignment.
+ * Backward: dx [rows][C] packed; dw, db [C] or NULL; workspace of ppv_layernorm_bwd_workspace_bytes (needed where dw or db is asked for).
+ * Deterministic. */
+int ppv_layernorm_fwd(const void* x, long ldx, const void* w, const void* b, void* y, float* mean, float* rstd, long rows, int C, int dtype,
+                      int wdtype, float eps, ppv_stream_t stream);
+size_t ppv_layernorm_bwd_workspace_bytes(long rows, int C, int dtype);
+int ppv_layernorm_bwd(const void* g, long ldg, const void* x, long ldx, const void* w, const float* mean, const float* rstd, void* dx, void* dw,
+                      void* db, void* workspace, long rows, int C, int dtype, int wdtype, ppv_stream_t stream);
+
 /* weight gradient (layer2..4 trainable, models.py:43-54): torch layout [N][Cs][R][S] f32 out; per-slice slabs in scratch */
 size_t ppv_conv_wgrad_scratch_bytes(long M, int N, int R, int S, int Cs);
 int ppv_conv_wgrad(const void* G, const void* X, float* dW_out, void* scratch, const void* zero_page, int B, int Hs,

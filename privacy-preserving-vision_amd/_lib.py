@@ -1,5 +1,6 @@
 """ctypes binding of libppv_hip.so (include/ppv_hip.h).  The product path has NO fallback:
 if the shared object is missing or a symbol is absent, importing a kernel wrapper raises."""
+import contextlib
 import ctypes
 import os
 import re
@@ -13,7 +14,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "ppv_hip.h")
 _c = ctypes
 _P, _I, _L, _F, _Z = _c.c_void_p, _c.c_int, _c.c_long, _c.c_float, _c.c_size_t
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 PPV_ERR_NULL, PPV_ERR_BAD_SIZE, PPV_ERR_INIT, PPV_ERR_WORKSPACE = -1001, -1002, -1003, -1004   # include/ppv_hip.h
 
 # name -> (restype, argtypes); mirrors include/ppv_hip.h (tests check the two agree)
@@ -108,6 +109,10 @@ PROTOTYPES = {
     "ppv_conv_gemm_red": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P] + [_I] * 13 + [_P]),
     "ppv_weight_layout_multi": (_I, [_P, _I, _I, _P]),
     "ppv_adam_multi": (_I, [_P, _I, _I] + [_c.c_double] * 7 + [_P]),
+    "ppv_adamw_multi": (_I, [_P, _I, _I] + [_c.c_double] * 6 + [_c.c_uint, _P]),
+    "ppv_layernorm_fwd": (_I, [_P, _L, _P, _P, _P, _P, _P, _L, _I, _I, _I, _F, _P]),
+    "ppv_layernorm_bwd_workspace_bytes": (_Z, [_L, _I, _I]),
+    "ppv_layernorm_bwd": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P]),
     "ppv_weight_layout": (_I, [_P, _P, _I, _I, _I, _I, _I, _P]),
     "ppv_conv_stat_tiles": (_I, [_L]),
     "ppv_conv_bn_relu_coop": (_I, [_P] * 10 + [_F, _F, _P, _P] + [_I] * 6 + [_P]),
@@ -251,6 +256,15 @@ def stream_ptr():
     if _raw_stream is not None and _cur_device is not None:
         return ctypes.c_void_p(_raw_stream(_cur_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_same_device = contextlib.nullcontext()
+
+
+def device_of(t):
+    """Context in which ``t``'s device is the current one (``stream_ptr`` and every launch go to the current device)."""
+    i = t.device.index
+    return _same_device if i is None or i == (_cur_device() if _cur_device is not None else torch.cuda.current_device()) else torch.cuda.device(i)
 
 
 def ptr(t):

@@ -1,0 +1,388 @@
+// Layer norm over the last axis, forward and backward with the weight gradient's reduction (gfx950).
+//
+//     mean = sum_c x / C,  rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps),  h = (x - mean) rstd,  y = h w + b
+//     dx = rstd (g w - mean_c(g w) - h mean_c(g w h)),  dw = sum_rows g h,  db = sum_rows g
+//
+// Byte-bound: forward reads x and writes y, backward reads x and g and writes dx, once each.  A row is held in registers by LPR lanes
+// (16, a wave, or a workgroup), NV 16-byte vectors each, so the variance is the two-pass one (sum of squared distances from the mean: no
+// cancellation for rows far from zero) without reading the row again.  All sums are f32.  Rows may start at any element: the 16-byte
+// loads ask for element alignment only (global memory takes them), the last vector of a row is taken element by element.
+// Backward: a fixed grid strides over the rows, every lane keeps the weight-gradient sums of its columns in registers, a workgroup
+// leaves one partial row, a second launch adds the partial rows in their order (no atomics: the same bits every time).
+#include <hip/hip_runtime.h>
+#include <hip/hip_fp16.h>
+#include "ppv_common.h"
+#include "ppv_hip.h"
+#include "elem_types.h"
+
+namespace ppv {
+
+// sum over the LPR lanes of a row's group, the same value (same order of additions) in each of them
+template <int LPR> __device__ __forceinline__ float group_sum(float v, float* lds) {
+    v = row16_sum_f(v);
+    if constexpr (LPR >= 64) v = wave_sum_of_rows(v);
+    if constexpr (LPR > 64) {
+        constexpr int NW = LPR / 64;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) v += lds[i];
+        __syncthreads();                                       // the next sum writes the same words
+    }
+    return v;
+}
+
+template <class T, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__ x, long ldx, const void* __restrict__ w, const void* __restrict__ b,
+                                                           int wdtype, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                                                           long rows, int C, float eps) {
+    constexpr int V = 16 / sizeof(T), RPW = NT / LPR;
+    __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
+    const int l = threadIdx.x % LPR;
+    const long row = (long)blockIdx.x * RPW + threadIdx.x / LPR;
+    const bool live = row < rows;                              // (a dead group keeps running: the sums below cross lanes)
+    const T* xr = x + (live ? row : 0) * ldx;
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + l) * V;
+        load_vec<T, V>(xr + c, C - c, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += v[i][e];
+    const float inv_c = 1.f / (float)C;
+    const float mean = group_sum<LPR>(s, lds) * inv_c;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int left = C - (i * LPR + l) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            v[i][e] = e < left ? v[i][e] - mean : 0.f;
+            q = __builtin_fmaf(v[i][e], v[i][e], q);
+        }
+    }
+    const float rstd = 1.f / __builtin_sqrtf(group_sum<LPR>(q, lds) * inv_c + eps);
+    if (!live) return;
+    T* yr = y + row * (long)C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + l) * V;
+        if (c >= C) continue;
+        float wv[V], bv[V], o[V];
+        load_param<V>(w, wdtype, c, C - c, 1.f, wv);
+        load_param<V>(b, wdtype, c, C - c, 0.f, bv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(v[i][e] * rstd, wv[e], bv[e]);
+        store_vec<T, V>(yr + c, C - c, o);
+    }
+    if (mean_out && l == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
+}
+
+// rows longer than the registers hold: three passes over the row (the second and third come out of the L2)
+template <class T>
+__global__ __launch_bounds__(256) void layernorm_fwd_long_kernel(const T* __restrict__ x, long ldx, const void* __restrict__ w, const void* __restrict__ b,
+                                                                 int wdtype, T* __restrict__ y, float* __restrict__ mean_out,
+                                                                 float* __restrict__ rstd_out, int C, float eps) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ float lds[4];
+    const long row = blockIdx.x;
+    const T* xr = x + row * ldx;
+    float v[V];
+    float s = 0.f, q = 0.f;
+    for (int c = threadIdx.x * V; c < C; c += 256 * V) {
+        load_vec<T, V>(xr + c, C - c, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += v[e];
+    }
+    const float mean = group_sum<256>(s, lds) / (float)C;
+    for (int c = threadIdx.x * V; c < C; c += 256 * V) {
+        load_vec<T, V>(xr + c, C - c, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = e < C - c ? v[e] - mean : 0.f;
+            q = __builtin_fmaf(d, d, q);
+        }
+    }
+    const float rstd = 1.f / __builtin_sqrtf(group_sum<256>(q, lds) / (float)C + eps);
+    T* yr = y + row * (long)C;
+    for (int c = threadIdx.x * V; c < C; c += 256 * V) {
+        float wv[V], bv[V];
+        load_vec<T, V>(xr + c, C - c, v);
+        load_param<V>(w, wdtype, c, C - c, 1.f, wv);
+        load_param<V>(b, wdtype, c, C - c, 0.f, bv);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = __builtin_fmaf((v[e] - mean) * rstd, wv[e], bv[e]);
+        store_vec<T, V>(yr + c, C - c, v);
+    }
+    if (mean_out && threadIdx.x == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
+}
+
+template <class T, int LPR, int NV, int NT>
+__global__ __launch_bounds__(NT) void layernorm_bwd_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
+                                                           const void* __restrict__ w, int wdtype, const float* __restrict__ mean_in,
+                                                           const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
+                                                           long rows, int C) {
+    constexpr int V = 16 / sizeof(T), RPW = NT / LPR;
+    extern __shared__ float smem[];                            // [2][C] partial sums (LPR <= 64), then the words of group_sum
+    __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
+    const int l = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + l) * V;
+        load_param<V>(w, wdtype, c, C - c, 1.f, wv[i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) aw[i][e] = ab[i][e] = 0.f;
+    }
+    const float inv_c = 1.f / (float)C;
+    const long step = (long)gridDim.x * RPW, turns = (rows + step - 1) / step;
+    for (long t = 0; t < turns; ++t) {                         // the same number of turns for every lane: the sums cross lanes and waves
+        const long row = t * step + (long)blockIdx.x * RPW + grp;
+        const bool live = row < rows;
+        const long at = live ? row : 0;
+        float gv[NV][V], hv[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            load_vec<T, V>(g + at * ldg + c, live ? C - c : 0, gv[i]);
+            load_vec<T, V>(x + at * ldx + c, live ? C - c : 0, hv[i]);
+        }
+        const float mean = mean_in[at], rstd = rstd_in[at];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int left = live ? C - (i * LPR + l) * V : 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float h = e < left ? (hv[i][e] - mean) * rstd : 0.f, gw = gv[i][e] * wv[i][e];   // (g is zero behind the row)
+                aw[i][e] = __builtin_fmaf(gv[i][e], h, aw[i][e]);
+                ab[i][e] += gv[i][e];
+                s1 += gw;
+                s2 = __builtin_fmaf(gw, h, s2);
+                hv[i][e] = h;
+                gv[i][e] = gw;
+            }
+        }
+        s1 = group_sum<LPR>(s1, lds) * inv_c;
+        s2 = group_sum<LPR>(s2, lds) * inv_c;
+        if (!live) continue;
+        T* dr = dx + row * (long)C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            if (c >= C) continue;
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = rstd * (gv[i][e] - s1 - hv[i][e] * s2);
+            store_vec<T, V>(dr + c, C - c, o);
+        }
+    }
+    if (!part) return;
+    float* pw = part + (long)blockIdx.x * 2 * C;
+    if constexpr (LPR <= 64) {                                 // several rows at a time in this workgroup: their sums meet in LDS, in order
+        if constexpr (LPR < 64) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) { aw[i][e] = wave_sum_of_rows(aw[i][e]); ab[i][e] = wave_sum_of_rows(ab[i][e]); }
+        }
+        for (int wv_ = 0; wv_ < NT / 64; ++wv_) {
+            if ((int)(threadIdx.x >> 6) == wv_ && (threadIdx.x & 63) < LPR) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const int c = (i * LPR + l) * V + e;
+                        if (c < C) {
+                            smem[c] = wv_ ? smem[c] + aw[i][e] : aw[i][e];
+                            smem[C + c] = wv_ ? smem[C + c] + ab[i][e] : ab[i][e];
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < 2 * C; c += NT) pw[c] = smem[c];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int c = (i * LPR + l) * V + e;
+                if (c < C) { pw[c] = aw[i][e]; pw[C + c] = ab[i][e]; }
+            }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void layernorm_bwd_long_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
+                                                                 const void* __restrict__ w, int wdtype, const float* __restrict__ mean_in,
+                                                                 const float* __restrict__ rstd_in, T* __restrict__ dx, int C) {
+    constexpr int V = 16 / sizeof(T);
+    __shared__ float lds[4];
+    const long row = blockIdx.x;
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int c = threadIdx.x * V; c < C; c += 256 * V) {
+            float gv[V], xv[V], wv[V];
+            load_vec<T, V>(g + row * ldg + c, C - c, gv);
+            load_vec<T, V>(x + row * ldx + c, C - c, xv);
+            load_param<V>(w, wdtype, c, C - c, 1.f, wv);
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float h = e < C - c ? (xv[e] - mean) * rstd : 0.f, gw = gv[e] * wv[e];
+                if (pass == 0) { s1 += gw; s2 = __builtin_fmaf(gw, h, s2); }
+                o[e] = rstd * (gw - s1 - h * s2);
+            }
+            if (pass == 1) store_vec<T, V>(dx + row * (long)C + c, C - c, o);
+        }
+        if (pass == 0) {
+            s1 = group_sum<256>(s1, lds) / (float)C;
+            s2 = group_sum<256>(s2, lds) / (float)C;
+        }
+    }
+}
+
+// weight-gradient partials of the long rows: a thread owns a column, a workgroup row of the grid strides over the rows
+template <class T>
+__global__ __launch_bounds__(256) void layernorm_wgrad_long_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
+                                                                   const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                                                                   float* __restrict__ part, long rows, int C) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    float aw = 0.f, ab = 0.f;
+    for (long r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float gv = to_f32(g[r * ldg + c]);
+        aw = __builtin_fmaf(gv, (to_f32(x[r * ldx + c]) - mean_in[r]) * rstd_in[r], aw);
+        ab += gv;
+    }
+    part[(long)blockIdx.y * 2 * C + c] = aw;
+    part[(long)blockIdx.y * 2 * C + C + c] = ab;
+}
+
+// part [G][2][C] -> dw, db: 16 columns x 16 slices of the partial rows per workgroup, the slices added in order
+__global__ __launch_bounds__(256) void layernorm_wgrad_reduce_kernel(const float* __restrict__ part, int G, int C, void* __restrict__ dw,
+                                                                     void* __restrict__ db, int wdtype) {
+    __shared__ float s[16][17];
+    const int j = threadIdx.x & 15, k = threadIdx.x >> 4;
+    const long c = (long)blockIdx.x * 16 + j;                  // over the 2 C columns of a partial row
+    float a = 0.f;
+    if (c < 2L * C) {
+#pragma unroll 4
+        for (int r = k; r < G; r += 16) a += part[(long)r * 2 * C + c];
+    }
+    s[k][j] = a;
+    __syncthreads();
+    if (k == 0 && c < 2L * C) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) a += s[i][j];
+        void* out = c < C ? dw : db;
+        if (out) store_param(out, wdtype, c < C ? c : c - C, a);
+    }
+}
+
+// workgroups of the backward pass: enough to fill the chip, at least four rows for each row slot, so that the partial rows stay few
+static int layernorm_bwd_groups(long rows, int C, int rpw) {
+    const long by_rows = (rows + 4L * rpw - 1) / (4L * rpw);
+    const long most = C > 16384 ? 64 : 512;
+    return (int)(by_rows < 1 ? 1 : by_rows > most ? most : by_rows);
+}
+// vectors of a row -> lanes per row of the backward kernels (at most 32 elements a lane: two gradient sums, a weight and two operands each)
+static int layernorm_bwd_lpr(int C, int dtype) {
+    const int v = dtype == 0 ? 4 : 8, nvec = (C + v - 1) / v, most = 32 / v;
+    return nvec <= 16 ? 16 : nvec <= 64 * most ? 64 : nvec <= 256 * most ? 256 : nvec <= 512 * most ? 512 : 0;
+}
+static int layernorm_groups_of(long rows, int C, int dtype) {
+    const int lpr = layernorm_bwd_lpr(C, dtype);
+    return layernorm_bwd_groups(rows, C, lpr == 16 ? 16 : lpr == 64 ? 4 : 1);
+}
+
+template <class T>
+static int layernorm_fwd_t(const T* x, long ldx, const void* w, const void* b, int wdtype, T* y, float* mean, float* rstd, long rows, int C,
+                           float eps, hipStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const int nvec = (C + V - 1) / V;
+    auto grid = [&](int rpw) { return (rows + rpw - 1) / rpw; };
+    if (grid(16) > 0x7fffffffL || (nvec > 16 && grid(4) > 0x7fffffffL) || (nvec > 512 && rows > 0x7fffffffL)) return PPV_ERR_BAD_SIZE;
+#define LN_FWD(LPR, NV, NT) \
+    layernorm_fwd_kernel<T, LPR, NV, NT><<<(unsigned)grid(NT / LPR), NT, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, rows, C, eps)
+    if (nvec <= 16) LN_FWD(16, 1, 256);
+    else if (nvec <= 64) LN_FWD(64, 1, 256);
+    else if (nvec <= 128) LN_FWD(64, 2, 256);
+    else if (nvec <= 256) LN_FWD(64, 4, 256);
+    else if (nvec <= 512) LN_FWD(64, 8, 256);
+    else if (nvec <= 1024) LN_FWD(256, 4, 256);
+    else if (nvec <= 2048) LN_FWD(256, 8, 256);
+    else layernorm_fwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, C, eps);
+#undef LN_FWD
+    return ppv_last_error();
+}
+
+template <class T>
+static int layernorm_bwd_t(const T* g, long ldg, const T* x, long ldx, const void* w, int wdtype, const float* mean, const float* rstd, T* dx,
+                           void* dw, void* db, float* part, long rows, int C, int dtype, hipStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const int nvec = (C + V - 1) / V, lpr = layernorm_bwd_lpr(C, dtype), G = layernorm_groups_of(rows, C, dtype);
+    if (!dw && !db) part = nullptr;
+#define LN_BWD(LPR, NV, NT) \
+    layernorm_bwd_kernel<T, LPR, NV, NT><<<G, NT, LPR <= 64 ? 2 * C * sizeof(float) : 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, part, rows, C)
+    if (lpr == 16) LN_BWD(16, 1, 256);
+    else if (lpr == 64) {
+        if (nvec <= 64) LN_BWD(64, 1, 256);
+        else if (nvec <= 128) LN_BWD(64, 2, 256);
+        else if (nvec <= 256) LN_BWD(64, 4, 256);
+        else LN_BWD(64, 32 / V, 256);                          // (f32 only: 8 vectors; the 16-bit types end at 4)
+    } else if (lpr == 256) {
+        if (nvec <= 512) LN_BWD(256, 2, 256);
+        else if (nvec <= 1024) LN_BWD(256, 4, 256);
+        else LN_BWD(256, 32 / V, 256);
+    } else if (lpr == 512) LN_BWD(512, 32 / V, 512);
+    else {
+        if (rows > 0x7fffffffL) return PPV_ERR_BAD_SIZE;
+        layernorm_bwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, C);
+        if (part) layernorm_wgrad_long_kernel<T><<<dim3((C + 255) / 256, G), 256, 0, stream>>>(g, ldg, x, ldx, mean, rstd, part, rows, C);
+    }
+#undef LN_BWD
+    if (part) layernorm_wgrad_reduce_kernel<<<(unsigned)((2L * C + 15) / 16), 256, 0, stream>>>(part, G, C, dw, db, wdtype);
+    return ppv_last_error();
+}
+
+}  // namespace ppv
+
+using namespace ppv;
+
+extern "C" {
+
+int ppv_layernorm_fwd(const void* x, long ldx, const void* w, const void* b, void* y, float* mean, float* rstd, long rows, int C, int dtype,
+                      int wdtype, float eps, hipStream_t stream) {
+    if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return PPV_ERR_NULL;
+    if (rows < 1 || C < 1 || C > (1 << 30) || ldx < 0 || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return PPV_ERR_BAD_SIZE;
+    if (dtype == 0) return layernorm_fwd_t((const float*)x, ldx, w, b, wdtype, (float*)y, mean, rstd, rows, C, eps, stream);
+    if (dtype == 1) return layernorm_fwd_t((const bf16s*)x, ldx, w, b, wdtype, (bf16s*)y, mean, rstd, rows, C, eps, stream);
+    return layernorm_fwd_t((const f16s*)x, ldx, w, b, wdtype, (f16s*)y, mean, rstd, rows, C, eps, stream);
+}
+
+size_t ppv_layernorm_bwd_workspace_bytes(long rows, int C, int dtype) {
+    if (rows < 1 || C < 1 || C > (1 << 30) || dtype < 0 || dtype > 2) return 0;
+    return (size_t)layernorm_groups_of(rows, C, dtype) * 2 * (size_t)C * sizeof(float);
+}
+
+int ppv_layernorm_bwd(const void* g, long ldg, const void* x, long ldx, const void* w, const float* mean, const float* rstd, void* dx, void* dw,
+                      void* db, void* workspace, long rows, int C, int dtype, int wdtype, hipStream_t stream) {
+    if (!g || !x || !mean || !rstd || !dx || ((dw || db) && !workspace)) return PPV_ERR_NULL;
+    if (rows < 1 || C < 1 || C > (1 << 30) || ldx < 0 || ldg < 0 || dtype < 0 || dtype > 2 || wdtype < 0 || wdtype > 2) return PPV_ERR_BAD_SIZE;
+    float* part = (float*)workspace;
+    if (dtype == 0)
+        return layernorm_bwd_t((const float*)g, ldg, (const float*)x, ldx, w, wdtype, mean, rstd, (float*)dx, dw, db, part, rows, C, dtype, stream);
+    if (dtype == 1)
+        return layernorm_bwd_t((const bf16s*)g, ldg, (const bf16s*)x, ldx, w, wdtype, mean, rstd, (bf16s*)dx, dw, db, part, rows, C, dtype, stream);
+    return layernorm_bwd_t((const f16s*)g, ldg, (const f16s*)x, ldx, w, wdtype, mean, rstd, (f16s*)dx, dw, db, part, rows, C, dtype, stream);
+}
+
+}  // extern "C"

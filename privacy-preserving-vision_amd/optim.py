@@ -4,7 +4,9 @@ Reference use: the harness' optimisers, ``Image_Caption/train.py:92-101`` (``tor
 encoder.parameters()), lr=encoder_lr)`` and the decoder's twin), stepped at ``train.py:318-321``.  Same constructor arguments, same
 ``param_groups`` / ``state`` layout (``step``, ``exp_avg``, ``exp_avg_sq`` per parameter, so ``state_dict()`` loads into
 ``torch.optim.Adam`` and back), same arithmetic as torch's fused kernel in f32 (``csrc/optim.hip``).  Not supported and refused loudly:
-``amsgrad``, ``maximize``, ``capturable``, sparse or non-f32 gradients.  No CPU / stock-torch fallback: the HIP library does the step."""
+``amsgrad``, ``maximize``, ``capturable``, sparse or non-f32 gradients.  No CPU / stock-torch fallback: the HIP library does the step.
+
+``ppv_amd.optim.AdamW``: torch.optim.AdamW (decoupled weight decay) the same way, with its moments in 32 or in 8 bits (``csrc/adamw.hip``)."""
 import struct
 
 import numpy as np
@@ -92,4 +94,151 @@ class Adam(torch.optim.Optimizer):
                                             1.0 - b1 ** n, 1.0 - b2 ** n, _lib.stream_ptr()), "ppv_adam_multi")
                 for p in sub:
                     self.state[p]["step"] += 1
+        return loss
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW(params, lr, betas, eps, weight_decay) with every tensor of a group updated in one launch.
+
+    ``state_bits=32``: ``exp_avg`` and ``exp_avg_sq`` in f32; ``state_dict()`` loads into torch.optim.AdamW and back.
+
+    ``state_bits=8``: tensors of at least ``min_8bit_size`` elements keep 2 bytes of state per parameter instead of 8 (the smaller ones, biases
+    and norm weights, stay in 32 bits): ``exp_avg`` and ``exp_avg_sq_root`` (the root of the second moment) as float8_e4m3fn, each with one
+    f32 power-of-two scale per 256 consecutive elements (``exp_avg_scale``, ``exp_avg_sq_root_scale``; value = code * scale).  The new
+    moments are computed in f32 and rounded stochastically, up with the probability of the upper neighbour's nearness: to the nearest, a second moment
+    that moves by a thousandth per step would never leave its code.  The random numbers are a hash of ``seed``, the step, the tensor's
+    place in the optimiser and the element's place in the tensor: the same run gives the same bits.
+
+    Parameters and gradients are contiguous f32 tensors of one GPU per group; parameters without a gradient are left alone and keep their own
+    step count (a float).  Refused: amsgrad, maximize, capturable, sparse gradients, and a step inside a stream capture (the step's number is part of
+    the launch, a replay would repeat it)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False, capturable=False,
+                 state_bits=32, min_8bit_size=4096, seed=0):
+        if amsgrad or maximize or capturable:
+            raise NotImplementedError("ppv_amd.optim.AdamW: amsgrad / maximize / capturable are not implemented")
+        if not 0.0 <= lr or not 0.0 <= eps or not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or not 0.0 <= weight_decay:
+            raise ValueError("ppv_amd.optim.AdamW: invalid hyper-parameter")
+        if state_bits not in (8, 32):
+            raise ValueError("ppv_amd.optim.AdamW: state_bits is 8 or 32")
+        if min_8bit_size < 0:
+            raise ValueError("ppv_amd.optim.AdamW: min_8bit_size >= 0")
+        self.state_bits, self.min_8bit_size, self.seed = state_bits, min_8bit_size, int(seed)
+        self._tables = {}                      # (group index, slot) -> (the addresses it holds, descriptor table on the device, its blocks)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
+                                      foreach=None, capturable=False, differentiable=False, fused=None))
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        for st in self.state.values():
+            for k, x in st.items():            # own copies: the moments are updated in place, and the given state may be another optimiser's
+                if k == "step":
+                    st[k] = float(x)
+                elif "exp_avg_scale" in st and not k.endswith("_scale"):
+                    st[k] = x.to(torch.float8_e4m3fn)     # torch has cast the 8-bit values to the parameter's f32, where each of them exists
+                else:
+                    st[k] = x.clone(memory_format=torch.contiguous_format)
+        self._tables = {}
+
+    def __getstate__(self):
+        st = super().__getstate__()
+        st.update(state_bits=self.state_bits, min_8bit_size=self.min_8bit_size, seed=self.seed)
+        return st
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._number()
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        self._number()
+
+    def _number(self):
+        self._place = {p: i for i, p in enumerate(p for g in self.param_groups for p in g["params"])}
+        self._tables = {}
+
+    def _init_state(self, p):
+        st = self.state[p]
+        st["step"] = 0.0
+        if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+            for k in ("exp_avg", "exp_avg_sq_root"):
+                st[k] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                st[k + "_scale"] = torch.zeros((p.numel() + 255) // 256, dtype=torch.float32, device=p.device)
+        else:
+            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+
+    @staticmethod
+    def _moments(st):
+        """(m, v, scale of m, scale of v) of a parameter's state: which form it has is the state's own affair (it may have been loaded)."""
+        if "exp_avg_scale" in st:
+            return st["exp_avg"], st["exp_avg_sq_root"], st["exp_avg_scale"], st["exp_avg_sq_root_scale"]
+        return st["exp_avg"], st["exp_avg_sq"], None, None
+
+    def _table(self, slot, ps):
+        moments = [self._moments(self.state[p]) for p in ps]
+        # every address that the records hold is in the key (and the stream that the table was written on): another one, another table
+        key = [p.data_ptr() for p in ps] + [p.grad.data_ptr() for p in ps] + [t.data_ptr() for m in moments for t in m if t is not None]
+        key.append(_lib.stream_ptr().value)
+        hit = self._tables.get(slot)
+        if hit is not None and hit[0] == key:
+            return hit[1], hit[2], hit[3]
+        recs, blk = [], 0
+        for p, (m, v, ms, vs) in zip(ps, moments):
+            n = p.numel()
+            if n == 0:
+                continue
+            ok = all(t.device == p.device and t.is_contiguous() and t.numel() == n for t in (m, v))
+            if ms is None:
+                ok = ok and m.dtype == v.dtype == torch.float32
+            else:
+                ok = ok and m.dtype == v.dtype == torch.float8_e4m3fn and all(
+                    t.device == p.device and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == (n + 255) // 256 for t in (ms, vs))
+            if not ok:
+                raise ValueError("ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)")
+            recs.append(struct.pack("<QQQQQQqiI", p.data_ptr(), p.grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms.data_ptr() if ms is not None else 0,
+                                    vs.data_ptr() if vs is not None else 0, n, blk, self._place[p] & 0xFFFFFFFF))
+            blk += (n + _CHUNK - 1) // _CHUNK
+        desc = None
+        if recs:                               # pinned and non-blocking: a list whose gradients move every step does not wait for the device
+            desc = torch.frombuffer(bytearray(b"".join(recs)), dtype=torch.uint8).pin_memory().to(ps[0].device, non_blocking=True)
+        self._tables[slot] = (key, desc, len(recs), blk)
+        return desc, len(recs), blk
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        L = _lib.lib()
+        f32, strided = torch.float32, torch.strided
+        for gi, group in enumerate(self.param_groups):
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            dev = ps[0].device
+            for p in ps:
+                g = p.grad
+                if (g.dtype is not f32 or p.dtype is not f32 or g.layout is not strided or not g.is_contiguous() or not p.is_contiguous()
+                        or p.device != dev or g.device != dev or g.numel() != p.numel() or dev.type != "cuda"):
+                    raise NotImplementedError("ppv_amd.optim.AdamW: contiguous f32 parameters and gradients on one GPU only")
+                if not self.state[p]:
+                    self._init_state(p)
+            with _lib.device_of(ps[0]):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("ppv_amd.optim.AdamW: a step cannot be captured into a graph (its number is part of the launch)")
+                by_step = {}                   # parameters whose gradient was missing in some step keep their own count
+                for p in ps:
+                    by_step.setdefault(float(self.state[p]["step"]), []).append(p)
+                for k in [k for k in self._tables if k[0] == gi and k[1] >= len(by_step)]:
+                    del self._tables[k]
+                b1, b2 = group["betas"]
+                for slot, (t, sub) in enumerate(sorted(by_step.items())):
+                    desc, n, blocks = self._table((gi, slot), sub)
+                    if n:
+                        _lib.check(L.ppv_adamw_multi(desc.data_ptr(), n, blocks, float(group["lr"]), b1, b2, group["eps"], group["weight_decay"],
+                                                     t + 1.0, self.seed & 0xFFFFFFFF, _lib.stream_ptr()), "ppv_adamw_multi")
+                    for p in sub:
+                        self.state[p]["step"] = t + 1.0
         return loss

@@ -1,0 +1,300 @@
+"""ppv_amd.optim.AdamW (csrc/adamw.hip), moments in 32 and in 8 bits.  The step is a stated sequence of f32 operations, so the oracle's values
+(oracle/transformer.py, f32 on the CPU) are reproduced bit for bit; against 64 bits the bounds count roundings."""
+import copy
+import math
+import pickle
+
+import pytest
+import torch
+
+from oracle import transformer as orc
+
+U = 2.0 ** -24
+SIZES = [(64,), (5,), (4095,), (4096,), (4099,), (64, 3, 7, 7), (300, 257), (1,), (12288,), (7, 4096)]
+
+
+def _tensors(seed, sizes, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g) * scale for s in sizes]
+
+
+def _oracle_state(n, eight):
+    z = lambda k: torch.zeros(k)
+    b = -(-n // 256)
+    return {"m": z(n), "r": z(n), "ms": z(b), "rs": z(b)} if eight else {"m": z(n), "v": z(n)}
+
+
+def _same(opt, p, st):
+    got = opt.state[p]
+    if "r" in st:
+        pairs = [(got["exp_avg"].float(), st["m"]), (got["exp_avg_sq_root"].float(), st["r"]), (got["exp_avg_scale"], st["ms"]),
+                 (got["exp_avg_sq_root_scale"], st["rs"])]
+    else:
+        pairs = [(got["exp_avg"], st["m"]), (got["exp_avg_sq"], st["v"])]
+    for a, b in pairs:
+        a = a.cpu().reshape(-1)
+        assert torch.equal(torch.nan_to_num(a, nan=-12345.0), torch.nan_to_num(b, nan=-12345.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("wd,betas", [(0.0, (0.9, 0.999)), (1e-2, (0.8, 0.95))])
+def test_adamw_reproduces_the_oracle_bit_for_bit(bits, wd, betas):
+    from ppv_amd.optim import AdamW
+    ref = [t.reshape(-1) for t in _tensors(0, SIZES)]
+    got = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, SIZES)]
+    st = [_oracle_state(r.numel(), bits == 8 and r.numel() >= 4096) for r in ref]
+    count = [0] * len(ref)
+    opt = AdamW(got, lr=1e-2, betas=betas, weight_decay=wd, state_bits=bits, seed=11)
+    flat = torch.zeros(sum(r.numel() for r in ref) + 3, device="cuda")             # gradients are slices of one buffer, few of them aligned
+    for step in range(6):
+        grads = _tensors(100 + step, SIZES, scale=10.0 ** (-step))                 # (the blocks' maxima move through powers of two)
+        grads[4][:] = 0.0 if step < 2 else grads[4]                                # no gradient at all at first
+        off = 1
+        for i, (q, g) in enumerate(zip(got, grads)):
+            view = flat[off:off + g.numel()].view_as(g)
+            view.copy_(g)
+            off += g.numel()
+            q.grad = None if (step == 3 and i in (3, 6)) else view                # a parameter without a gradient keeps its own count
+        opt.step()
+        for i, (r, g) in enumerate(zip(ref, grads)):
+            if got[i].grad is None:
+                continue
+            count[i] += 1
+            orc.adamw_step(r, g.reshape(-1), st[i], count[i], place=i, lr=1e-2, betas=betas, weight_decay=wd, seed=11)
+            assert opt.state[got[i]]["step"] == count[i]
+            _same(opt, got[i], st[i])
+            assert torch.equal(got[i].detach().cpu().reshape(-1), r), (step, i)
+    assert (bits == 8) == any(s.get("exp_avg_scale") is not None for s in opt.state.values())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wd", [0.0, 1e-2])
+def test_adamw_32_against_64_bits_and_torch(wd):
+    """Five steps from zero moments against the formula in f64.  A step rounds m and v at most 3 times each on operands no larger than
+    |m| + |g| (v: 3 |v|), the errors shrink by the betas: after t steps at most 4 t u (|m| + max|g|) and 4 t u v.  The update lr m / r^ inherits
+    their relative errors plus 8 of its own roundings; p is rounded twice per step."""
+    from ppv_amd.optim import AdamW
+    p0 = _tensors(1, [(513,), (70, 70)])
+    got = [torch.nn.Parameter(t.cuda()) for t in p0]
+    tor = [torch.nn.Parameter(t.double()) for t in p0]
+    opt, ref = AdamW(got, lr=1e-2, weight_decay=wd), torch.optim.AdamW(tor, lr=1e-2, weight_decay=wd, foreach=False)
+    for step in range(5):
+        for q, t, g in zip(got, tor, _tensors(50 + step, [(513,), (70, 70)])):
+            q.grad, t.grad = g.cuda(), g.double()
+        opt.step()
+        ref.step()
+    t = 5
+    for q, r in zip(got, tor):
+        a, b = opt.state[q], ref.state[r]
+        assert ((a["exp_avg"].cpu().double() - b["exp_avg"]).abs() <= 4 * t * U * (b["exp_avg"].abs() + 5.0)).all()
+        assert ((a["exp_avg_sq"].cpu().double() - b["exp_avg_sq"]).abs() <= 4 * t * U * b["exp_avg_sq"] + 1e-30).all()
+        # |update| <= lr * 10 (|m^| <= sqrt(v^) / sqrt(1 - b1 ...) of a few steps), m's absolute error seen through 1 / r^ >= 1 / 5
+        small = torch.sqrt(b["exp_avg_sq"] / (1 - 0.999 ** t)).clamp(min=1e-3)
+        tol = 2 * t * U * r.detach().abs() + t * 1e-2 * (16 * t * U * 10 + 4 * t * U * 10 / small)
+        assert ((q.detach().cpu().double() - r.detach()).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_adamw_loads_aligned_or_not_and_leaves_the_neighbours():
+    """Parameters that are slices of a buffer at every offset: the elements between them are not touched."""
+    from ppv_amd.optim import AdamW
+    buf, grad = torch.randn(40000, device="cuda"), torch.randn(40000, device="cuda")
+    before = buf.clone()
+    spans = [(1, 4096), (4099, 5000), (9103, 1), (9106, 8192), (17299, 12287), (29589, 9000)]
+    ps = []
+    for at, n in spans:
+        p = buf[at:at + n].requires_grad_(True)
+        p.grad = grad[at:at + n]
+        ps.append(p)
+    AdamW(ps, lr=1e-2, state_bits=8).step()
+    inside = torch.zeros(40000, dtype=torch.bool)
+    for at, n in spans:
+        inside[at:at + n] = True
+    b, a = before.cpu(), buf.detach().cpu()
+    assert torch.equal(a[~inside], b[~inside]) and (a[inside] != b[inside]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_state_survives_reload_and_pickle(bits):
+    """Rolled back to a saved state the same steps give the same bits; the saved state is not what later steps write to."""
+    from ppv_amd.optim import AdamW
+    sizes = [(300,), (64, 128), (4099,)]
+    got = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, sizes)]
+    opt = AdamW(got, lr=1e-2, state_bits=bits, seed=3)
+
+    def run(o, a, b):
+        for s in range(a, b):
+            for q, g in zip(got, _tensors(200 + s, sizes)):
+                q.grad = g.cuda()
+            o.step()
+
+    run(opt, 0, 2)
+    sd = opt.state_dict()
+    kept = copy.deepcopy(sd)
+    w = [q.detach().clone() for q in got]
+    run(opt, 2, 5)
+    want = [q.detach().clone() for q in got]
+    fresh = AdamW(got, lr=1e-2, state_bits=bits, seed=3)
+    for o in (opt, fresh, pickle.loads(pickle.dumps(AdamW([torch.nn.Parameter(torch.zeros(1))], state_bits=bits, seed=3)))):
+        if o is not opt and o is not fresh:
+            assert (o.state_bits, o.seed, o.min_8bit_size) == (bits, 3, 4096) and o._tables == {}
+            continue
+        with torch.no_grad():
+            for q, x in zip(got, w):
+                q.copy_(x)
+        o.load_state_dict(kept)
+        run(o, 2, 5)
+        assert all(torch.equal(a, b.detach()) for a, b in zip(want, got))
+    again = copy.deepcopy(opt.state_dict())                    # `kept` itself is as it was saved
+    assert kept["state"][0]["step"] == 2.0 and again["state"][0]["step"] == 5.0
+    if bits == 8:
+        st = kept["state"][1]
+        assert st["exp_avg"].dtype == torch.float8_e4m3fn and st["exp_avg"].shape == (64, 128) and st["exp_avg_scale"].shape == (32,)
+        assert opt.state[got[1]]["exp_avg"].dtype == torch.float8_e4m3fn
+    else:
+        t = torch.optim.AdamW(got, lr=1e-2)
+        t.load_state_dict(kept)                                # interchangeable with torch's
+        back = AdamW(got, lr=1e-2)
+        back.load_state_dict(t.state_dict())
+        assert torch.equal(back.state[got[2]]["exp_avg_sq"], kept["state"][2]["exp_avg_sq"])
+
+
+@pytest.mark.gpu
+def test_adamw_8bit_values_that_are_not_finite_stay_where_they_are():
+    from ppv_amd.optim import AdamW
+    n = 8192
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = AdamW([p], lr=1e-2, state_bits=8, seed=1)
+    ref, st = torch.zeros(n), _oracle_state(n, True)
+    for step in range(3):
+        g = torch.randn(n, generator=torch.Generator().manual_seed(step))
+        if step == 1:
+            g[5], g[700], g[4000] = math.inf, math.nan, -math.inf
+        p.grad = g.cuda()
+        opt.step()
+        orc.adamw_step(ref, g, st, step + 1, lr=1e-2, seed=1)
+        _same(opt, p, st)
+    bad = ~torch.isfinite(p.detach().cpu())
+    assert bad.nonzero().squeeze(1).tolist() == [5, 700, 4000]
+    assert torch.equal(p.detach().cpu()[~bad], ref[~bad])
+
+
+@pytest.mark.gpu
+def test_adamw_on_two_streams_and_with_moving_gradients():
+    """The descriptor table follows the stream and the gradients' addresses."""
+    from ppv_amd.optim import AdamW
+    sizes = [(5000,), (64, 64)]
+    a = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, sizes)]
+    b = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, sizes)]
+    oa, ob = AdamW(a, lr=1e-2, state_bits=8), AdamW(b, lr=1e-2, state_bits=8)
+    side, keep = torch.cuda.Stream(), []
+    for step in range(6):
+        grads = [g.cuda() for g in _tensors(step, sizes)]
+        keep.append(grads)                                      # new addresses every step
+        for p, g in zip(a, grads):
+            p.grad = g
+        oa.step()
+        for p, g in zip(b, grads):
+            p.grad = g.clone()
+        torch.cuda.synchronize()
+        if step % 2:
+            with torch.cuda.stream(side):
+                ob.step()
+            side.synchronize()
+        else:
+            ob.step()
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and len(ob._tables) == 1
+
+
+def test_8bit_second_moment_follows_a_constant_gradient():
+    """Why the rounding is stochastic (the format alone, on the CPU): with g = 1 and beta2 = 0.999 the second moment is 1 - 0.999^t.  A step of the
+    root is at most 2^-3 of it and moves it by at most its own share d <= 0.5e-3 / r^2, so rounding adds at most (2^-3 r) (d r) per step to
+    E[r^2], against a decay of 1e-3: at most 6.3 % too much in v.  To the nearest, the root stops where half a step of e4m3 (>= 2^-5 of it)
+    is more than an update: below 0.2."""
+    n, steps = 2048, 2500
+    for nearest in (False, True):
+        st, p, g = _oracle_state(n, True), torch.zeros(n), torch.ones(n)
+        if nearest:
+            keep = orc.dither
+            orc.dither = lambda seed, step, place, k: (torch.full((k,), 32767), torch.full((k,), 32767))
+        try:
+            for t in range(1, steps + 1):
+                orc.adamw_step(p, g, st, t, lr=0.0)
+        finally:
+            if nearest:
+                orc.dither = keep
+        v = ((st["r"] * orc.spread(st["rs"], n)).double() ** 2).mean().item()
+        want = 1 - 0.999 ** steps
+        if nearest:
+            assert v < 0.2
+        else:
+            assert 0.98 * want <= v <= 1.063 * want + 0.02
+
+
+def test_adamw_refusals():
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in ({"amsgrad": True}, {"maximize": True}, {"capturable": True}):
+        with pytest.raises(NotImplementedError):
+            AdamW([p], **kw)
+    for kw in ({"state_bits": 16}, {"lr": -1.0}, {"betas": (1.0, 0.9)}, {"betas": (0.9, -0.1)}, {"eps": -1e-8}, {"weight_decay": -0.1},
+               {"min_8bit_size": -1}):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(TypeError):
+        AdamW([p], nesterov=True)
+    o = AdamW([p])
+    o.step()                                                    # nothing has a gradient: nothing to do
+    p.grad = torch.zeros(4)
+    with pytest.raises(NotImplementedError):
+        o.step()                                                # no CPU path
+
+
+def test_adamw_entry_point_refuses():
+    import ctypes
+    from ppv_amd import _lib
+    L, p = _lib.lib(), ctypes.c_void_p(64)
+    NULL, SIZE = _lib.PPV_ERR_NULL, _lib.PPV_ERR_BAD_SIZE
+    hyper = (1e-3, 0.9, 0.999, 1e-8, 0.0)
+    assert L.ppv_adamw_multi(None, 1, 1, *hyper, 1.0, 0, None) == NULL
+    assert L.ppv_adamw_multi(p, 0, 1, *hyper, 1.0, 0, None) == SIZE
+    assert L.ppv_adamw_multi(p, 1, 0, *hyper, 1.0, 0, None) == SIZE
+    assert L.ppv_adamw_multi(p, 1, 1, *hyper, 0.0, 0, None) == SIZE
+    assert L.ppv_adamw_multi(p, 1, 1, 1e-3, 1.0, 0.999, 1e-8, 0.0, 1.0, 0, None) == SIZE
+    assert L.ppv_adamw_multi(p, 1, 1, 1e-3, 0.9, 1.5, 1e-8, 0.0, 1.0, 0, None) == SIZE
+
+
+@pytest.mark.gpu
+def test_adamw_refuses_on_the_gpu():
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(8, 8, device="cuda"))
+    p.grad = torch.zeros(8, 8, device="cuda").t()
+    with pytest.raises(NotImplementedError):
+        AdamW([p]).step()
+    p.grad = torch.zeros(8, 8, device="cuda")
+    o = AdamW([p])
+    o.step()
+    o.state[p]["exp_avg"] = torch.zeros(3, device="cuda")
+    with pytest.raises(ValueError):
+        o.step()
+    e = torch.nn.Parameter(torch.zeros(0, device="cuda"))
+    e.grad = torch.zeros(0, device="cuda")
+    o = AdamW([e])
+    o.step()
+    assert o.state[e]["step"] == 1.0
+    q = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    q.grad = torch.ones(8, device="cuda")
+    o = AdamW([q])
+    o.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    refused = False
+    with torch.cuda.graph(graph):
+        scratch = torch.empty(4, device="cuda").zero_()         # (a capture that holds something)
+        try:
+            o.step()
+        except RuntimeError:
+            refused = True
+    assert refused and o.state[q]["step"] == 1.0 and scratch.numel() == 4
