@@ -239,6 +239,31 @@ size_t ppv_layernorm_bwd_workspace_bytes(long rows, int C, int dtype);
 int ppv_layernorm_bwd(const void* g, long ldg, const void* x, long ldx, const void* w, const float* mean, const float* rstd, void* dx, void* dw,
                       void* db, void* workspace, long rows, int C, int dtype, int wdtype, ppv_stream_t stream);
 
+/* ---- multi-head attention (csrc/attention.hip, csrc/attention_bwd.hip) -----------------------------
+ * out = softmax(scale q k^T over the visible keys) v.  q, dout [B][Tq][H][D] and k, v [B][Tk][Hkv][D] by their strides in elements (batch, token,
+ * head; the last axis has stride 1); out, dq [B][Tq][H][D] and dk, dv [B][Tk][Hkv][D] packed.  H is a multiple of Hkv: query head h reads
+ * key head h / (H / Hkv).  dtype 0 f32, 1 bf16, 2 f16 of all of them; D <= 128 and every stride a multiple of 16 bytes, every address too.
+ * q_lens, k_lens: DEVICE int32 [B] or NULL (Tq, Tk); values are clamped to 0..Tq, 0..Tk.  Row i < q_len sees key j < k_len, where causal if
+ * j <= i + k_len - q_len.  Rows at or behind q_len and rows that see nothing give zeros (and zero gradients); keys at or behind k_len are
+ * not read and get zero gradients.  lse [B][H][Tq] f32: log2 of the softmax's denominator, written by the forward pass (or NULL) and read by the
+ * backward pass, as is out.  workspace: of ppv_attention_fwd_workspace_bytes (may be 0) / ppv_attention_bwd_workspace_bytes. */
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    const void* dout;
+    void *dq, *dk, *dv;
+    void* workspace;
+    const int *q_lens, *k_lens;
+    long sqb, sqt, sqh, skb, skt, skh, svb, svt, svh, sgb, sgt, sgh;
+    int B, H, Hkv, Tq, Tk, D, dtype, causal;
+    float scale;
+} PpvAttention;
+size_t ppv_attention_fwd_workspace_bytes(int B, int H, int Hkv, int Tq, int Tk, int D, int dtype);
+int ppv_attention_fwd(const PpvAttention* x, ppv_stream_t stream);
+size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Tq);
+int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream);
+
 /* weight gradient (layer2..4 trainable, models.py:43-54): torch layout [N][Cs][R][S] f32 out; per-slice slabs in scratch */
 size_t ppv_conv_wgrad_scratch_bytes(long M, int N, int R, int S, int Cs);
 int ppv_conv_wgrad(const void* G, const void* X, float* dW_out, void* scratch, const void* zero_page, int B, int Hs,

@@ -14,7 +14,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "ppv_hip.h")
 _c = ctypes
 _P, _I, _L, _F, _Z = _c.c_void_p, _c.c_int, _c.c_long, _c.c_float, _c.c_size_t
 
-ABI_VERSION = 22
+ABI_VERSION = 23
 PPV_ERR_NULL, PPV_ERR_BAD_SIZE, PPV_ERR_INIT, PPV_ERR_WORKSPACE = -1001, -1002, -1003, -1004   # include/ppv_hip.h
 
 # name -> (restype, argtypes); mirrors include/ppv_hip.h (tests check the two agree)
@@ -189,6 +189,19 @@ class WgradReduce(ctypes.Structure):
 
 PROTOTYPES["ppv_conv_wgrad_ex"] = (_I, [_P, _P, _P, _P, _P] + [_I] * 11 + [_P, ctypes.POINTER(WgradReduce)])
 PROTOTYPES["ppv_wgrad_reduce_multi"] = (_I, [ctypes.POINTER(WgradReduce), _I, _P])
+
+
+class Attention(ctypes.Structure):
+    """include/ppv_hip.h PpvAttention."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "workspace", "q_lens", "k_lens")]
+                + [(n, _L) for n in ("sqb", "sqt", "sqh", "skb", "skt", "skh", "svb", "svt", "svh", "sgb", "sgt", "sgh")]
+                + [(n, _I) for n in ("B", "H", "Hkv", "Tq", "Tk", "D", "dtype", "causal")] + [("scale", _F)])
+
+
+PROTOTYPES["ppv_attention_fwd_workspace_bytes"] = (_Z, [_I] * 7)
+PROTOTYPES["ppv_attention_fwd"] = (_I, [ctypes.POINTER(Attention), _P])
+PROTOTYPES["ppv_attention_bwd_workspace_bytes"] = (_Z, [_I] * 3)
+PROTOTYPES["ppv_attention_bwd"] = (_I, [ctypes.POINTER(Attention), _P])
 
 TRUNK_MAX_BLOCKS = 64
 

@@ -1,0 +1,312 @@
+// Multi-head attention, backward (gfx950).  P is computed again from Q, K and the saved log-sum-exp; nothing of size Tq x Tk is stored:
+//
+//     P = exp2(scale log2e Q K^T - lse),   dP = dO V^T,   D = rowsum(dO O),   dS = P (dP - D)
+//     dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
+//
+// Two launches, no atomics: the gradients have the same bits every time.
+//   attn_dq   a wave owns 32 rows (columns of S^T, dP^T, dQ^T) and walks over the keys; it also leaves D for the second launch
+//   attn_dkv  a wave owns 32 keys (columns of S, dP, dK^T, dV^T) and walks over the rows of all query heads that share them
+// That is 7 products where one launch with atomics on dQ would need 5.  Bound by the matrix pipe and, behind it, the LDS: every operand of a
+// tile is read along its rows (S, dP) and across them (dQ, dK, dV).
+#include "attention_tiles.h"
+
+namespace ppv {
+
+struct AttnBwd {
+    AttnDims d;
+    AttnTensor q, k, v, g;                                     // g: dO
+    const void* out;
+    const float* lse;                                          // [B][H][Tq], log2
+    float* delta;                                              // [B][H][Tq]
+    void *dq, *dk, *dv;
+    int ntile;
+};
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
+    using TL = Tile<T, DP>;
+    constexpr int NT = NW * 64, KT = 32;
+    __shared__ __attribute__((aligned(16))) char smem[2][2][TL::bytes(KT)];
+    const AttnDims& d = a.d;
+    int bh, tile;
+    if (!attn_block(d, a.ntile, bh, tile)) return;
+    if (d.causal) tile = a.ntile - 1 - tile;
+    const int b = bh / d.Hkv, hk = bh - b * d.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int qlen = attn_len(d.q_lens, b, d.Tq), klen = attn_len(d.k_lens, b, d.Tk);
+    const int rows = qlen * d.G, shift = klen - qlen;
+    const int row0 = tile * NW * 32, row = row0 + wave * 32 + (lane & 31);
+    const int nch = d.D * TL::ES / 16;
+    const RowsOf<T> Q{(const T*)a.q.p + b * a.q.sb + (long)hk * d.G * a.q.sh, a.q.st, a.q.sh, d.G};
+    const RowsOf<T> GO{(const T*)a.g.p + b * a.g.sb + (long)hk * d.G * a.g.sh, a.g.st, a.g.sh, d.G};
+    const RowsOf<T> O{(const T*)a.out + ((long)b * d.Tq * d.H + hk * d.G) * d.D, (long)d.H * d.D, d.D, d.G};
+    const RowsOf<T> K{(const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, 0, 1};
+    const RowsOf<T> V{(const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, 0, 1};
+
+    const int tok = (int)((unsigned)row / (unsigned)d.G), tok0 = (int)((unsigned)row0 / (unsigned)d.G);
+    const int last = min(row0 + NW * 32, rows) - 1;
+    int kend = klen;
+    if (d.causal) kend = min(klen, max(0, (int)((unsigned)max(last, 0) / (unsigned)d.G) + shift + 1));
+    if (row0 >= rows) kend = 0;
+    const int ktiles = (kend + KT - 1) / KT;
+    const int lim = row < rows ? (d.causal ? min(klen - 1, tok + shift) : klen - 1) : -1;
+    const int lim0 = d.causal ? min(klen - 1, tok0 + shift) : klen - 1;
+
+    Stager<T, DP, KT, NT> sk, sv;
+    if (ktiles) {
+        sk.fetch(K, 0, klen, nch, tid);
+        sv.fetch(V, 0, klen, nch, tid);
+    }
+    u32x4 qf[TL::NF], gf[TL::NF];
+    load_own<T, DP>(qf, Q, row, rows, nch, lane);
+    load_own<T, DP>(gf, GO, row, rows, nch, lane);
+    float delta = 0.f;
+    {
+        u32x4 of[TL::NF];
+        load_own<T, DP>(of, O, row, rows, nch, lane);
+#pragma unroll
+        for (int kd = 0; kd < TL::NF; ++kd) {
+            float x[16 / TL::ES], y[16 / TL::ES];
+            unpack_vec<T>(of[kd], x);
+            unpack_vec<T>(gf[kd], y);
+#pragma unroll
+            for (int e = 0; e < 16 / TL::ES; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+        }
+    }
+    delta = half_swap_sum(delta);
+    const int h = hk * d.G + (row - tok * d.G);
+    const long stat = ((long)b * d.H + h) * d.Tq + tok;
+    float lse = 0.f;
+    if (row < rows) {
+        lse = a.lse[stat];
+        if (half == 0) a.delta[stat] = delta;
+    }
+    const float c = d.scale * LOG2E;
+    f32x16 acc[TL::DB];
+#pragma unroll
+    for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
+
+    for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= 1) {
+        char *tk = smem[buf][0], *tv = smem[buf][1];
+        sk.put(tk, tid);
+        sv.put(tv, tid);
+        __syncthreads();
+        if (kt + 1 < ktiles) {
+            sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
+            sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
+        }
+        f32x16 s, p;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
+#pragma unroll
+        for (int kd = 0; kd < TL::NF; ++kd) {
+            s = TL::mma(TL::by_row(tk, 0, kd, lane), qf[kd], s);
+            p = TL::mma(TL::by_row(tv, 0, kd, lane), gf[kd], p);
+        }
+        const bool hidden = kt * KT + KT - 1 > lim0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * (p[j] - delta);
+            if (hidden && kt * KT + 8 * (j >> 2) + 4 * half + (j & 3) > lim) ds = 0.f;
+            s[j] = ds;
+        }
+#pragma unroll
+        for (int kf = 0; kf < TL::CF; ++kf) {
+            const u32x4 df = TL::from_acc(s, kf);
+#pragma unroll
+            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, 0, i, kf, lane), df, acc[i]);
+        }
+    }
+    if (row >= d.Tq * d.G) return;
+#pragma unroll
+    for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] = lim < 0 ? 0.f : acc[i][j] * d.scale;      // (rows that see nothing: zeros, whatever K holds)
+    T* po = (T*)a.dq + (((long)b * d.Tq + tok) * d.H + h) * d.D;
+#pragma unroll
+    for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = i * 32 + g * 8 + half * 4;
+            if (e < d.D) store4<T>(po + e, acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]);
+        }
+}
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
+    using TL = Tile<T, DP>;
+    constexpr int NT = NW * 64, QT = 32;
+    __shared__ __attribute__((aligned(16))) char smem[2][2][TL::bytes(QT)];
+    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];      // lse, delta
+    __shared__ __attribute__((aligned(16))) int limit[2][QT];          // last key that a row sees
+    const AttnDims& d = a.d;
+    int bh, tile;
+    if (!attn_block(d, a.ntile, bh, tile)) return;
+    const int b = bh / d.Hkv, hk = bh - b * d.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int qlen = attn_len(d.q_lens, b, d.Tq), klen = attn_len(d.k_lens, b, d.Tk);
+    const int rows = qlen * d.G, shift = klen - qlen;
+    const int key0 = tile * NW * 32, key = key0 + wave * 32 + (lane & 31);
+    const int nch = d.D * TL::ES / 16;
+    const RowsOf<T> Q{(const T*)a.q.p + b * a.q.sb + (long)hk * d.G * a.q.sh, a.q.st, a.q.sh, d.G};
+    const RowsOf<T> GO{(const T*)a.g.p + b * a.g.sb + (long)hk * d.G * a.g.sh, a.g.st, a.g.sh, d.G};
+    const RowsOf<T> K{(const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, 0, 1};
+    const RowsOf<T> V{(const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, 0, 1};
+
+    // rows that see a key of this workgroup
+    const int first = d.causal ? max(0, key0 - shift) : 0;     // (token)
+    const int rt0 = key0 < klen ? (int)min((long)first * d.G, (long)rows) / QT : 0;
+    const int rt1 = key0 < klen ? (rows + QT - 1) / QT : 0;
+
+    Stager<T, DP, QT, NT> sq, sg;
+    float st = 0.f;
+    int sl = -1;
+    auto fetch = [&](int rt) {
+        sq.fetch(Q, rt * QT, rows, nch, tid);
+        sg.fetch(GO, rt * QT, rows, nch, tid);
+        // threads 0..31: lse and limit; 32..63: delta
+        if (tid < 64) {
+            const int r = rt * QT + (tid & 31), t = (int)((unsigned)r / (unsigned)d.G);
+            st = 0.f;
+            sl = -1;
+            if (r < rows) {
+                const long at = ((long)b * d.H + hk * d.G + (r - t * d.G)) * d.Tq + t;
+                st = tid < 32 ? a.lse[at] : a.delta[at];
+                sl = d.causal ? min(klen - 1, t + shift) : klen - 1;
+            }
+        }
+    };
+    if (rt0 < rt1) fetch(rt0);
+    u32x4 kf_[TL::NF], vf[TL::NF];
+    load_own<T, DP>(kf_, K, key, klen, nch, lane);
+    load_own<T, DP>(vf, V, key, klen, nch, lane);
+    const float c = d.scale * LOG2E;
+    f32x16 dk[TL::DB], dv[TL::DB];
+#pragma unroll
+    for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) dk[i][j] = dv[i][j] = 0.f;
+
+    for (int rt = rt0, buf = 0; rt < rt1; ++rt, buf ^= 1) {
+        char *tq = smem[buf][0], *tg = smem[buf][1];
+        sq.put(tq, tid);
+        sg.put(tg, tid);
+        if (tid < 64) {
+            stat[buf][tid >> 5][tid & 31] = st;
+            if (tid < 32) limit[buf][tid] = sl;
+        }
+        __syncthreads();
+        if (rt + 1 < rt1) fetch(rt + 1);
+        f32x16 s, p;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
+#pragma unroll
+        for (int kd = 0; kd < TL::NF; ++kd) {
+            s = TL::mma(TL::by_row(tq, 0, kd, lane), kf_[kd], s);
+            p = TL::mma(TL::by_row(tg, 0, kd, lane), vf[kd], p);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int r = 8 * g + 4 * half;
+            const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][0][r]), de = *reinterpret_cast<const float4*>(&stat[buf][1][r]);
+            const int4 li = *reinterpret_cast<const int4*>(&limit[buf][r]);
+            const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
+            const int liv[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 4 * g + i;
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lsv[i])), ds = pe * (p[j] - dev[i]);
+                const bool seen = key <= liv[i];
+                p[j] = seen ? pe : 0.f;
+                s[j] = seen ? ds : 0.f;
+            }
+        }
+#pragma unroll
+        for (int kf = 0; kf < TL::CF; ++kf) {
+            const u32x4 pf = TL::from_acc(p, kf), df = TL::from_acc(s, kf);
+#pragma unroll
+            for (int i = 0; i < TL::DB; ++i) {
+                dv[i] = TL::mma(TL::by_col(tg, 0, i, kf, lane), pf, dv[i]);
+                dk[i] = TL::mma(TL::by_col(tq, 0, i, kf, lane), df, dk[i]);
+            }
+        }
+    }
+    if (key >= d.Tk) return;
+    const long at = (((long)b * d.Tk + key) * d.Hkv + hk) * d.D;
+#pragma unroll
+    for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = i * 32 + g * 8 + half * 4;
+            if (e < d.D) {
+                store4<T>((T*)a.dk + at + e, dk[i][4 * g] * d.scale, dk[i][4 * g + 1] * d.scale, dk[i][4 * g + 2] * d.scale, dk[i][4 * g + 3] * d.scale);
+                store4<T>((T*)a.dv + at + e, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+            }
+        }
+}
+
+static int attn_waves(long n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
+
+template <class T, int DP> static int attn_bwd_t(AttnBwd a, hipStream_t stream) {
+    const long rows = (long)a.d.Tq * a.d.G;
+    // (f32 at 128: one wave alone would have to hold more of a tile in flight than it has registers)
+    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;
+    const int nq = attn_waves(rows) < LEAST ? LEAST : attn_waves(rows), nk = attn_waves(a.d.Tk) < LEAST ? LEAST : attn_waves(a.d.Tk);
+    a.ntile = (int)((rows + nq * 32 - 1) / (nq * 32));
+    const int tk = (a.d.Tk + nk * 32 - 1) / (nk * 32);
+    if ((long)a.d.nbh * a.ntile > 0x7ffffff0L || (long)a.d.nbh * tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
+    unsigned grid = attn_grid(a.d, a.ntile);
+    if (nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, LEAST * 64, 0, stream>>>(a);
+    else if (nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 128, 0, stream>>>(a);
+    else attn_dq_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
+    if (a.d.Tk == 0) return ppv_last_error();
+    a.ntile = tk;
+    grid = attn_grid(a.d, tk);
+    if (nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, LEAST * 64, 0, stream>>>(a);
+    else if (nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 128, 0, stream>>>(a);
+    else attn_dkv_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
+    return ppv_last_error();
+}
+template <class T> static int attn_bwd_dp(const AttnBwd& a, hipStream_t stream) {
+    return a.d.D <= 32 ? attn_bwd_t<T, 32>(a, stream) : a.d.D <= 64 ? attn_bwd_t<T, 64>(a, stream) : attn_bwd_t<T, 128>(a, stream);
+}
+
+}  // namespace ppv
+
+using namespace ppv;
+
+extern "C" {
+
+size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Tq) {
+    return B < 1 || H < 1 || Tq < 1 ? 0 : (size_t)B * H * Tq * sizeof(float);
+}
+
+int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
+    if (!x) return PPV_ERR_NULL;
+    AttnBwd a = {};
+    if (int e = attn_check(x, &a.d)) return e;
+    if (!x->lse || !x->dout || !x->dq || !x->dk || !x->dv) return PPV_ERR_NULL;
+    if (!x->workspace) return PPV_ERR_WORKSPACE;
+    const int v = x->dtype == 0 ? 4 : 8;
+    const long st[] = {x->sgb, x->sgt, x->sgh};
+    for (long s : st)
+        if (s < 0 || s % v) return PPV_ERR_BAD_SIZE;
+    const void* ps[] = {x->dout, x->dq, x->dk, x->dv};
+    for (const void* p : ps)
+        if ((size_t)p % 16) return PPV_ERR_BAD_SIZE;
+    a.q = {x->q, x->sqb, x->sqt, x->sqh};
+    a.k = {x->k, x->skb, x->skt, x->skh};
+    a.v = {x->v, x->svb, x->svt, x->svh};
+    a.g = {x->dout, x->sgb, x->sgt, x->sgh};
+    a.out = x->out;
+    a.lse = x->lse;
+    a.delta = (float*)x->workspace;
+    a.dq = x->dq;
+    a.dk = x->dk;
+    a.dv = x->dv;
+    return x->dtype == 0 ? attn_bwd_dp<float>(a, stream) : x->dtype == 1 ? attn_bwd_dp<bf16s>(a, stream) : attn_bwd_dp<f16s>(a, stream);
+}
+
+}  // extern "C"
