@@ -246,10 +246,11 @@ int ppv_layernorm_bwd(const void* g, long ldg, const void* x, long ldx, const vo
  * q_lens, k_lens: DEVICE int32 [B] or NULL (Tq, Tk); values are clamped to 0..Tq, 0..Tk.  Row i < q_len sees key j < k_len, where causal if
  * j <= i + k_len - q_len.  Rows at or behind q_len and rows that see nothing give zeros (and zero gradients); keys at or behind k_len are
  * not read and get zero gradients.  lse [B][H][Tq] f32: log2 of the softmax's denominator, written by the forward pass (or NULL) and read by the
- * backward pass, as is out.  workspace: of ppv_attention_fwd_workspace_bytes (may be 0) / ppv_attention_bwd_workspace_bytes. */
+ * backward pass, as is out.  out_lo: packed like out, or NULL: what rounding to a 16-bit type took from out, written by the forward pass and read
+ * by the backward pass (which without it works with the rounded out).  workspace: of ppv_attention_fwd_workspace_bytes (may be 0) / ppv_attention_bwd_workspace_bytes. */
 typedef struct {
     const void *q, *k, *v;
-    void* out;
+    void *out, *out_lo;
     float* lse;
     const void* dout;
     void *dq, *dk, *dv;

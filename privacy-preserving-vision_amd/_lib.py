@@ -193,7 +193,7 @@ PROTOTYPES["ppv_wgrad_reduce_multi"] = (_I, [ctypes.POINTER(WgradReduce), _I, _P
 
 class Attention(ctypes.Structure):
     """include/ppv_hip.h PpvAttention."""
-    _fields_ = ([(n, _P) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "workspace", "q_lens", "k_lens")]
+    _fields_ = ([(n, _P) for n in ("q", "k", "v", "out", "out_lo", "lse", "dout", "dq", "dk", "dv", "workspace", "q_lens", "k_lens")]
                 + [(n, _L) for n in ("sqb", "sqt", "sqh", "skb", "skt", "skh", "svb", "svt", "svh", "sgb", "sgt", "sgh")]
                 + [(n, _I) for n in ("B", "H", "Hkv", "Tq", "Tk", "D", "dtype", "causal")] + [("scale", _F)])
 

@@ -33,10 +33,10 @@ def _strides(t):
     return tuple(0 if n == 1 else s for s, n in zip(t.stride()[:3], t.shape[:3]))
 
 
-def _describe(q, k, v, out, lse, q_lens, k_lens, causal, scale):
+def _describe(q, k, v, out, lo, lse, q_lens, k_lens, causal, scale):
     a = _lib.Attention()
-    a.q, a.k, a.v, a.out, a.lse = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr()
-    a.q_lens, a.k_lens = (None if t is None else t.data_ptr() for t in (q_lens, k_lens))
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.out_lo, a.lse, a.q_lens, a.k_lens = (None if t is None else t.data_ptr() for t in (lo, lse, q_lens, k_lens))
     (a.sqb, a.sqt, a.sqh), (a.skb, a.skt, a.skh), (a.svb, a.svt, a.svh) = _strides(q), _strides(k), _strides(v)
     a.B, a.Tq, a.H, a.D = q.shape
     a.Tk, a.Hkv = k.shape[1], k.shape[2]
@@ -50,39 +50,41 @@ def _padded(D, dtype):
 
 
 def _forward(q, k, v, q_lens, k_lens, causal, scale, keep):
-    """-> (out [B,Tq,H,D padded], lse or None, the operands as the kernels read them)."""
+    """-> (out [B,Tq,H,D padded], what rounding took from it or None, lse or None, the operands as the kernels read them).
+    keep: for a backward pass, whose rowsum(dO O) would carry the rounding of a 16-bit O into every score's gradient."""
     B, Tq, H, D = q.shape
     Dp = _padded(D, q.dtype)
     q, k, v = (_operand(t, Dp) for t in (q, k, v))
     out = torch.empty((B, Tq, H, Dp), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H, Tq), dtype=torch.float32, device=q.device) if keep else None
+    lo = torch.empty_like(out) if keep and q.dtype != torch.float32 else None
     if out.numel() == 0:
-        return out, lse, q, k, v
+        return out, lo, lse, q, k, v
     if k.numel() == 0:                                           # no keys at all: every row is empty
         out.zero_()
-        return out, lse, q, k, v
+        return out, lo, lse, q, k, v
     L = _lib.lib()
-    a = _describe(q, k, v, out, lse, q_lens, k_lens, causal, scale)
+    a = _describe(q, k, v, out, lo, lse, q_lens, k_lens, causal, scale)
     n = int(L.ppv_attention_fwd_workspace_bytes(a.B, a.H, a.Hkv, a.Tq, a.Tk, a.D, a.dtype))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     a.workspace = None if ws is None else ws.data_ptr()
     with _lib.device_of(q):
         check(L.ppv_attention_fwd(a, stream_ptr()), "ppv_attention_fwd")
-    return out, lse, q, k, v
+    return out, lo, lse, q, k, v
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_lens, k_lens, causal, scale):
-        out, lse, qp, kp, vp = _forward(q, k, v, q_lens, k_lens, causal, scale, True)
-        ctx.save_for_backward(qp, kp, vp, out, lse, q_lens, k_lens)
+        out, lo, lse, qp, kp, vp = _forward(q, k, v, q_lens, k_lens, causal, scale, True)
+        ctx.save_for_backward(qp, kp, vp, out, lo, lse, q_lens, k_lens)
         ctx.cfg = (causal, scale, q.shape[3])
         return out if out.shape[3] == q.shape[3] else out[..., :q.shape[3]].contiguous()
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
+        q, k, v, out, lo, lse, q_lens, k_lens = ctx.saved_tensors
         causal, scale, D = ctx.cfg
         Dp = out.shape[3]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -92,7 +94,7 @@ class _AttentionFn(torch.autograd.Function):
         else:
             L = _lib.lib()
             g = _operand(g, Dp)
-            a = _describe(q, k, v, out, lse, q_lens, k_lens, causal, scale)
+            a = _describe(q, k, v, out, lo, lse, q_lens, k_lens, causal, scale)
             a.dout, a.dq, a.dk, a.dv = g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
             a.sgb, a.sgt, a.sgh = _strides(g)
             ws = torch.empty(int(L.ppv_attention_bwd_workspace_bytes(a.B, a.H, a.Tq)), dtype=torch.uint8, device=q.device)

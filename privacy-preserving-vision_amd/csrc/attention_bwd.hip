@@ -15,36 +15,67 @@ namespace ppv {
 struct AttnBwd {
     AttnDims d;
     AttnTensor q, k, v, g;                                     // g: dO
-    const void* out;
+    const void *out, *out_lo;
     const float* lse;                                          // [B][H][Tq], log2
     float* delta;                                              // [B][H][Tq]
     void *dq, *dk, *dv;
     int ntile;
 };
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
+// four waves: OG groups that own 32 columns each x SG groups that divide a staged tile's rows, whose sums meet in LDS at the end
+template <class T, int DP, int OG, int ACC> struct BwdShape {
+    static constexpr int SG = 4 / OG, KT = 32 * SG;
+    static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
+    static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
+    static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
+    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG == 1 || ACC == 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG == 1 ? 1 : 2;
+};
+// adds the other groups' accumulators to the first one's (in their order); false: this wave is done
+template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* acc, float* lds, int og, int sg, int lane) {
+    if constexpr (SG > 1) {
+        float* park = lds + og * (SG - 1) * DB * 16 * 64 + lane;
+        if (sg > 0)
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) park[((sg - 1) * DB * 16 + i * 16 + j) * 64] = acc[i][j];
+        __syncthreads();
+        if (sg > 0) return false;
+#pragma unroll
+        for (int g = 0; g < SG - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[i][j] += park[(g * DB * 16 + i * 16 + j) * 64];
+    }
+    return true;
+}
+
+template <class T, int DP, int OG>
+__global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_kernel(const AttnBwd a) {
     using TL = Tile<T, DP>;
-    constexpr int NT = NW * 64, KT = 32;
-    __shared__ __attribute__((aligned(16))) char smem[2][2][TL::bytes(KT)];
+    using SH = BwdShape<T, DP, OG, 1>;
+    constexpr int NT = 256, KT = SH::KT, NB = SH::NB, SG = SH::SG;
+    __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
     const AttnDims& d = a.d;
     int bh, tile;
     if (!attn_block(d, a.ntile, bh, tile)) return;
     if (d.causal) tile = a.ntile - 1 - tile;
     const int b = bh / d.Hkv, hk = bh - b * d.Hkv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, og = wave % OG, sg = wave / OG;
     const int qlen = attn_len(d.q_lens, b, d.Tq), klen = attn_len(d.k_lens, b, d.Tk);
     const int rows = qlen * d.G, shift = klen - qlen;
-    const int row0 = tile * NW * 32, row = row0 + wave * 32 + (lane & 31);
+    const int row0 = tile * OG * 32, row = row0 + og * 32 + (lane & 31);
     const int nch = d.D * TL::ES / 16;
     const RowsOf<T> Q{(const T*)a.q.p + b * a.q.sb + (long)hk * d.G * a.q.sh, a.q.st, a.q.sh, d.G};
     const RowsOf<T> GO{(const T*)a.g.p + b * a.g.sb + (long)hk * d.G * a.g.sh, a.g.st, a.g.sh, d.G};
-    const RowsOf<T> O{(const T*)a.out + ((long)b * d.Tq * d.H + hk * d.G) * d.D, (long)d.H * d.D, d.D, d.G};
+    const long o0 = ((long)b * d.Tq * d.H + hk * d.G) * d.D;
+    const RowsOf<T> O{(const T*)a.out + o0, (long)d.H * d.D, d.D, d.G}, OL{(const T*)a.out_lo + o0, (long)d.H * d.D, d.D, d.G};
     const RowsOf<T> K{(const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, 0, 1};
     const RowsOf<T> V{(const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, 0, 1};
 
     const int tok = (int)((unsigned)row / (unsigned)d.G), tok0 = (int)((unsigned)row0 / (unsigned)d.G);
-    const int last = min(row0 + NW * 32, rows) - 1;
+    const int last = min(row0 + OG * 32, rows) - 1;
     int kend = klen;
     if (d.causal) kend = min(klen, max(0, (int)((unsigned)max(last, 0) / (unsigned)d.G) + shift + 1));
     if (row0 >= rows) kend = 0;
@@ -61,9 +92,9 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
     load_own<T, DP>(qf, Q, row, rows, nch, lane);
     load_own<T, DP>(gf, GO, row, rows, nch, lane);
     float delta = 0.f;
-    {
+    for (int part = 0; part < (a.out_lo ? 2 : 1); ++part) {   // O as the forward pass had it: its rounding would be dS's largest error
         u32x4 of[TL::NF];
-        load_own<T, DP>(of, O, row, rows, nch, lane);
+        load_own<T, DP>(of, part ? OL : O, row, rows, nch, lane);
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
             float x[16 / TL::ES], y[16 / TL::ES];
@@ -79,7 +110,7 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
     float lse = 0.f;
     if (row < rows) {
         lse = a.lse[stat];
-        if (half == 0) a.delta[stat] = delta;
+        if (half == 0 && sg == 0) a.delta[stat] = delta;
     }
     const float c = d.scale * LOG2E;
     f32x16 acc[TL::DB];
@@ -88,8 +119,10 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
 
-    for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= 1) {
-        char *tk = smem[buf][0], *tv = smem[buf][1];
+    const int own = sg * 32;                                   // this group's rows of a tile
+    for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= NB - 1) {
+        char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
+        if (NB == 1 && kt > 0) __syncthreads();
         sk.put(tk, tid);
         sv.put(tv, tid);
         __syncthreads();
@@ -102,23 +135,25 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
         for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
-            s = TL::mma(TL::by_row(tk, 0, kd, lane), qf[kd], s);
-            p = TL::mma(TL::by_row(tv, 0, kd, lane), gf[kd], p);
+            s = TL::mma(TL::by_row(tk, own, kd, lane), qf[kd], s);
+            p = TL::mma(TL::by_row(tv, own, kd, lane), gf[kd], p);
         }
         const bool hidden = kt * KT + KT - 1 > lim0;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * (p[j] - delta);
-            if (hidden && kt * KT + 8 * (j >> 2) + 4 * half + (j & 3) > lim) ds = 0.f;
+            if (hidden && kt * KT + own + 8 * (j >> 2) + 4 * half + (j & 3) > lim) ds = 0.f;
             s[j] = ds;
         }
 #pragma unroll
         for (int kf = 0; kf < TL::CF; ++kf) {
             const u32x4 df = TL::from_acc(s, kf);
 #pragma unroll
-            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, 0, i, kf, lane), df, acc[i]);
+            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, own, i, kf, lane), df, acc[i]);
         }
     }
+    if (SG > 1) __syncthreads();
+    if (!meet<TL::DB, OG, SG>(acc, (float*)smem, og, sg, lane)) return;
     if (row >= d.Tq * d.G) return;
 #pragma unroll
     for (int i = 0; i < TL::DB; ++i)
@@ -134,21 +169,22 @@ __global__ __launch_bounds__(NW * 64) void attn_dq_kernel(const AttnBwd a) {
         }
 }
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
+template <class T, int DP, int OG>
+__global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv_kernel(const AttnBwd a) {
     using TL = Tile<T, DP>;
-    constexpr int NT = NW * 64, QT = 32;
-    __shared__ __attribute__((aligned(16))) char smem[2][2][TL::bytes(QT)];
-    __shared__ __attribute__((aligned(16))) float stat[2][2][QT];      // lse, delta
-    __shared__ __attribute__((aligned(16))) int limit[2][QT];          // last key that a row sees
+    using SH = BwdShape<T, DP, OG, 1>;                         // (dK and dV meet one after the other)
+    constexpr int NT = 256, QT = SH::KT, NB = SH::NB, SG = SH::SG;
+    __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
+    __shared__ __attribute__((aligned(16))) float stat[NB][2][QT];     // lse, delta
+    __shared__ __attribute__((aligned(16))) int limit[NB][QT];         // last key that a row sees
     const AttnDims& d = a.d;
     int bh, tile;
     if (!attn_block(d, a.ntile, bh, tile)) return;
     const int b = bh / d.Hkv, hk = bh - b * d.Hkv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, og = wave % OG, sg = wave / OG;
     const int qlen = attn_len(d.q_lens, b, d.Tq), klen = attn_len(d.k_lens, b, d.Tk);
     const int rows = qlen * d.G, shift = klen - qlen;
-    const int key0 = tile * NW * 32, key = key0 + wave * 32 + (lane & 31);
+    const int key0 = tile * OG * 32, key = key0 + og * 32 + (lane & 31);
     const int nch = d.D * TL::ES / 16;
     const RowsOf<T> Q{(const T*)a.q.p + b * a.q.sb + (long)hk * d.G * a.q.sh, a.q.st, a.q.sh, d.G};
     const RowsOf<T> GO{(const T*)a.g.p + b * a.g.sb + (long)hk * d.G * a.g.sh, a.g.st, a.g.sh, d.G};
@@ -160,20 +196,21 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
     const int rt0 = key0 < klen ? (int)min((long)first * d.G, (long)rows) / QT : 0;
     const int rt1 = key0 < klen ? (rows + QT - 1) / QT : 0;
 
-    Stager<T, DP, QT, NT> sq, sg;
+    Stager<T, DP, QT, NT> sq, so;
     float st = 0.f;
     int sl = -1;
     auto fetch = [&](int rt) {
         sq.fetch(Q, rt * QT, rows, nch, tid);
-        sg.fetch(GO, rt * QT, rows, nch, tid);
-        // threads 0..31: lse and limit; 32..63: delta
-        if (tid < 64) {
-            const int r = rt * QT + (tid & 31), t = (int)((unsigned)r / (unsigned)d.G);
+        so.fetch(GO, rt * QT, rows, nch, tid);
+        // the first QT threads: lse and limit; the next QT: delta
+        static_assert(2 * QT <= NT, "a thread per statistic");
+        if (tid < 2 * QT) {
+            const int r = rt * QT + tid % QT, t = (int)((unsigned)r / (unsigned)d.G);
             st = 0.f;
             sl = -1;
             if (r < rows) {
                 const long at = ((long)b * d.H + hk * d.G + (r - t * d.G)) * d.Tq + t;
-                st = tid < 32 ? a.lse[at] : a.delta[at];
+                st = tid < QT ? a.lse[at] : a.delta[at];
                 sl = d.causal ? min(klen - 1, t + shift) : klen - 1;
             }
         }
@@ -189,13 +226,15 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) dk[i][j] = dv[i][j] = 0.f;
 
-    for (int rt = rt0, buf = 0; rt < rt1; ++rt, buf ^= 1) {
-        char *tq = smem[buf][0], *tg = smem[buf][1];
+    const int own = sg * 32;
+    for (int rt = rt0, buf = 0; rt < rt1; ++rt, buf ^= NB - 1) {
+        char *tq = smem + buf * 2 * TL::bytes(QT), *tg = tq + TL::bytes(QT);
+        if (NB == 1 && rt > rt0) __syncthreads();
         sq.put(tq, tid);
-        sg.put(tg, tid);
-        if (tid < 64) {
-            stat[buf][tid >> 5][tid & 31] = st;
-            if (tid < 32) limit[buf][tid] = sl;
+        so.put(tg, tid);
+        if (tid < 2 * QT) {
+            stat[buf][tid / QT][tid % QT] = st;
+            if (tid < QT) limit[buf][tid] = sl;
         }
         __syncthreads();
         if (rt + 1 < rt1) fetch(rt + 1);
@@ -204,12 +243,12 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
         for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
-            s = TL::mma(TL::by_row(tq, 0, kd, lane), kf_[kd], s);
-            p = TL::mma(TL::by_row(tg, 0, kd, lane), vf[kd], p);
+            s = TL::mma(TL::by_row(tq, own, kd, lane), kf_[kd], s);
+            p = TL::mma(TL::by_row(tg, own, kd, lane), vf[kd], p);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int r = 8 * g + 4 * half;
+            const int r = own + 8 * g + 4 * half;
             const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][0][r]), de = *reinterpret_cast<const float4*>(&stat[buf][1][r]);
             const int4 li = *reinterpret_cast<const int4*>(&limit[buf][r]);
             const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
@@ -228,11 +267,15 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
             const u32x4 pf = TL::from_acc(p, kf), df = TL::from_acc(s, kf);
 #pragma unroll
             for (int i = 0; i < TL::DB; ++i) {
-                dv[i] = TL::mma(TL::by_col(tg, 0, i, kf, lane), pf, dv[i]);
-                dk[i] = TL::mma(TL::by_col(tq, 0, i, kf, lane), df, dk[i]);
+                dv[i] = TL::mma(TL::by_col(tg, own, i, kf, lane), pf, dv[i]);
+                dk[i] = TL::mma(TL::by_col(tq, own, i, kf, lane), df, dk[i]);
             }
         }
     }
+    if (SG > 1) __syncthreads();
+    const bool first_group = meet<TL::DB, OG, SG>(dk, (float*)smem, og, sg, lane);
+    if (SG > 1) __syncthreads();
+    if (!meet<TL::DB, OG, SG>(dv, (float*)smem, og, sg, lane) || !first_group) return;
     if (key >= d.Tk) return;
     const long at = (((long)b * d.Tk + key) * d.Hkv + hk) * d.D;
 #pragma unroll
@@ -247,25 +290,24 @@ __global__ __launch_bounds__(NW * 64) void attn_dkv_kernel(const AttnBwd a) {
         }
 }
 
-static int attn_waves(long n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
+static int attn_groups(long n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 
 template <class T, int DP> static int attn_bwd_t(AttnBwd a, hipStream_t stream) {
     const long rows = (long)a.d.Tq * a.d.G;
-    // (f32 at 128: one wave alone would have to hold more of a tile in flight than it has registers)
-    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;
-    const int nq = attn_waves(rows) < LEAST ? LEAST : attn_waves(rows), nk = attn_waves(a.d.Tk) < LEAST ? LEAST : attn_waves(a.d.Tk);
+    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;  // (one group that holds K, V, dK and dV of 128 f32 spills)
+    const int nq = attn_groups(rows), nk = attn_groups(a.d.Tk) < LEAST ? LEAST : attn_groups(a.d.Tk);
     a.ntile = (int)((rows + nq * 32 - 1) / (nq * 32));
     const int tk = (a.d.Tk + nk * 32 - 1) / (nk * 32);
     if ((long)a.d.nbh * a.ntile > 0x7ffffff0L || (long)a.d.nbh * tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
     unsigned grid = attn_grid(a.d, a.ntile);
-    if (nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, LEAST * 64, 0, stream>>>(a);
-    else if (nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 128, 0, stream>>>(a);
+    if (nq == 1) attn_dq_kernel<T, DP, 1><<<grid, 256, 0, stream>>>(a);
+    else if (nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dq_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
     if (a.d.Tk == 0) return ppv_last_error();
     a.ntile = tk;
     grid = attn_grid(a.d, tk);
-    if (nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, LEAST * 64, 0, stream>>>(a);
-    else if (nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 128, 0, stream>>>(a);
+    if (nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
+    else if (nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dkv_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
     return ppv_last_error();
 }
@@ -301,6 +343,7 @@ int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
     a.v = {x->v, x->svb, x->svt, x->svh};
     a.g = {x->dout, x->sgb, x->sgt, x->sgh};
     a.out = x->out;
+    a.out_lo = x->out_lo;
     a.lse = x->lse;
     a.delta = (float*)x->workspace;
     a.dq = x->dq;
