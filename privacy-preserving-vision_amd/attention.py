@@ -20,7 +20,7 @@ def _operand(t, Dp):
     A view that is already so is taken as it is, any other is copied (zeros behind D add nothing to a product)."""
     v = 16 // t.element_size()
     if (t.shape[3] == Dp and t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(s % v == 0 or n == 1 for s, n in zip(t.stride()[:3], t.shape[:3]))):
+            and all(s % v == 0 or n == 1 for s, n in zip(t.stride()[:3], t.shape[:3])) and (t.stride(1) <= 1 << 22 or t.shape[1] == 1)):
         return t
     p = torch.empty(t.shape[:3] + (Dp,), dtype=t.dtype, device=t.device)
     if Dp != t.shape[3]:

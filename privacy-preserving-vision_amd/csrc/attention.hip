@@ -36,6 +36,7 @@ template <int KT> __device__ __forceinline__ void attn_units(const AttnDims& d, 
         for (int s = 1; s < 64; s <<= 1) t += __shfl_xor(t, s);
         total += t;
     }
+    total = __builtin_amdgcn_readfirstlane(total);
     per = max(2, (total + units - d.B - 1) / (units - d.B));   // sum of ceil(t / per) <= total / per + B <= units
     int before = 0;
     for (int i = 0; i < d.B; i += 64) {
@@ -49,13 +50,13 @@ template <int KT> __device__ __forceinline__ void attn_units(const AttnDims& d, 
         const int from = before + upto - n;
         const unsigned long long hit = __builtin_amdgcn_ballot_w64(find >= 0 ? find >= from && find < from + n : i + lane == b);
         if (hit) {
-            const int at = __builtin_ctzll(hit);
+            const int at = __builtin_ctzll(hit);               // (wave-uniform, and told so: the addresses that follow live in scalar registers)
             b = i + at;
-            first = __shfl(from, at);
-            count = __shfl(n, at);
+            first = __builtin_amdgcn_readlane(from, at);
+            count = __builtin_amdgcn_readlane(n, at);
             return;
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     if (find >= 0) b = -1;
 }
@@ -369,6 +370,7 @@ int attn_check(const PpvAttention* x, AttnDims* d) {
     const long st[] = {x->sqb, x->sqt, x->sqh, x->skb, x->skt, x->skh, x->svb, x->svt, x->svh};
     for (long s : st)
         if (s < 0 || s % v) return PPV_ERR_BAD_SIZE;
+    if (x->sqt > 1 << 22 || x->skt > 1 << 22 || x->svt > 1 << 22) return PPV_ERR_BAD_SIZE;      // (offsets inside a tile are 32 bits)
     const void* ps[] = {x->q, x->k, x->v, x->out, x->out_lo};
     for (const void* p : ps)
         if ((size_t)p % 16) return PPV_ERR_BAD_SIZE;

@@ -28,7 +28,7 @@ template <class T, int DP, int OG, int ACC> struct BwdShape {
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
-    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG == 1 || ACC == 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG == 1 ? 1 : 2;
+    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG == 1 || ACC == 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
 };
 // adds the other groups' accumulators to the first one's (in their order); false: this wave is done
 template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* acc, float* lds, int og, int sg, int lane) {
@@ -69,8 +69,6 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     const int nch = d.D * TL::ES / 16;
     const RowsOf<T> Q{(const T*)a.q.p + b * a.q.sb + (long)hk * d.G * a.q.sh, a.q.st, a.q.sh, d.G};
     const RowsOf<T> GO{(const T*)a.g.p + b * a.g.sb + (long)hk * d.G * a.g.sh, a.g.st, a.g.sh, d.G};
-    const long o0 = ((long)b * d.Tq * d.H + hk * d.G) * d.D;
-    const RowsOf<T> O{(const T*)a.out + o0, (long)d.H * d.D, d.D, d.G}, OL{(const T*)a.out_lo + o0, (long)d.H * d.D, d.D, d.G};
     const RowsOf<T> K{(const T*)a.k.p + b * a.k.sb + hk * a.k.sh, a.k.st, 0, 1};
     const RowsOf<T> V{(const T*)a.v.p + b * a.v.sb + hk * a.v.sh, a.v.st, 0, 1};
 
@@ -92,18 +90,23 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     load_own<T, DP>(qf, Q, row, rows, nch, lane);
     load_own<T, DP>(gf, GO, row, rows, nch, lane);
     float delta = 0.f;
-    for (int part = 0; part < (a.out_lo ? 2 : 1); ++part) {   // O as the forward pass had it: its rounding would be dS's largest error
+    auto dot = [&](const void* out) {
+        const RowsOf<T> O{(const T*)out + ((long)b * d.Tq * d.H + hk * d.G) * d.D, (long)d.H * d.D, d.D, d.G};
         u32x4 of[TL::NF];
-        load_own<T, DP>(of, part ? OL : O, row, rows, nch, lane);
+        load_own<T, DP>(of, O, row, rows, nch, lane);
+        float sum = 0.f;
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
             float x[16 / TL::ES], y[16 / TL::ES];
             unpack_vec<T>(of[kd], x);
             unpack_vec<T>(gf[kd], y);
 #pragma unroll
-            for (int e = 0; e < 16 / TL::ES; ++e) delta = __builtin_fmaf(x[e], y[e], delta);
+            for (int e = 0; e < 16 / TL::ES; ++e) sum = __builtin_fmaf(x[e], y[e], sum);
         }
-    }
+        return sum;
+    };
+    delta = dot(a.out);
+    if (a.out_lo) delta += dot(a.out_lo);                      // O as the forward pass had it: its rounding would be dS's largest error
     delta = half_swap_sum(delta);
     const int h = hk * d.G + (row - tok * d.G);
     const long stat = ((long)b * d.H + h) * d.Tq + tok;
@@ -335,6 +338,7 @@ int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
     const long st[] = {x->sgb, x->sgt, x->sgh};
     for (long s : st)
         if (s < 0 || s % v) return PPV_ERR_BAD_SIZE;
+    if (x->sgt > 1 << 22) return PPV_ERR_BAD_SIZE;
     const void* ps[] = {x->dout, x->dq, x->dk, x->dv};
     for (const void* p : ps)
         if ((size_t)p % 16) return PPV_ERR_BAD_SIZE;

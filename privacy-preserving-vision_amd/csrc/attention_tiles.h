@@ -153,13 +153,26 @@ template <class T, int DP, int ROWS, int NT> struct Stager {
     using TL = Tile<T, DP>;
     static constexpr int ALL = ROWS * TL::NCH, N = (ALL + NT - 1) / NT;
     static constexpr bool EVEN = N * NT == ALL;                // else: more threads than chunks
+    static_assert(NT % TL::NCH == 0, "a thread keeps its chunk");
+    static constexpr int STEP = NT / TL::NCH;                  // rows from one chunk of a thread to its next
     u32x4 v[N];
     __device__ __forceinline__ void fetch(const RowsOf<T>& src, int row0, int rows, int nch, int tid) {
+        const int r0 = tid / TL::NCH, ch = tid % TL::NCH;
+        const bool in = ch < nch;
+        if (src.G == 1) {                                      // a wave-uniform address and ONE 32-bit offset per lane (the strides are bounded)
+            const unsigned off = (unsigned)r0 * (unsigned)src.st * (unsigned)sizeof(T) + (unsigned)ch * 16u;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = i * NT + tid, r = row0 + idx / TL::NCH, ch = idx % TL::NCH;
-            if (r < rows && ch < nch && (EVEN || idx < ALL)) v[i] = *reinterpret_cast<const u32x4*>(src.row(r) + ch * (16 / (int)sizeof(T)));
-            else v[i] = (u32x4){0, 0, 0, 0};
+            for (int i = 0; i < N; ++i) {
+                const char* p = (const char*)(src.base + (long)(row0 + i * STEP) * src.st);
+                v[i] = in && row0 + i * STEP + r0 < rows && (EVEN || i * STEP + r0 < ROWS) ? *reinterpret_cast<const u32x4*>(p + off) : (u32x4){0, 0, 0, 0};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = row0 + i * STEP + r0;
+                v[i] = in && r < rows && (EVEN || i * STEP + r0 < ROWS) ? *reinterpret_cast<const u32x4*>(src.row(r) + ch * (16 / (int)sizeof(T)))
+                                                                        : (u32x4){0, 0, 0, 0};
+            }
         }
     }
     __device__ __forceinline__ void put(char* tile, int tid) const {
