@@ -1,7 +1,7 @@
 """ctypes binding of libppv_hip.so (include/ppv_hip.h).  The product path has NO fallback:
 if the shared object is missing or a symbol is absent, importing a kernel wrapper raises."""
-import contextlib
 import ctypes
+import importlib.util
 import os
 import re
 
@@ -9,6 +9,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PPV_LIB_PATH") or os.path.join(_HERE, "lib", "libppv_hip.so")   # override: A/B builds
+TORCH_LIB_PATH = os.path.join(_HERE, "lib", "ppv_torch.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "ppv_hip.h")
 
 _c = ctypes
@@ -254,6 +255,27 @@ def lib():
     return _lib
 
 
+_torch_ops = None
+_TORCH_ENTRIES = ("ppv_layernorm_fwd", "ppv_layernorm_bwd", "ppv_layernorm_bwd_workspace_bytes", "ppv_attention_fwd", "ppv_attention_fwd_workspace_bytes",
+                  "ppv_attention_bwd", "ppv_attention_bwd_workspace_bytes", "ppv_adamw_multi")
+
+
+def torch_ops():
+    """lib/ppv_torch.so (csrc/torch/torch_ops.cpp): the autograd nodes in C++, bound to the entry points of the loaded libppv_hip.so."""
+    global _torch_ops
+    if _torch_ops is None:
+        L = lib()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise RuntimeError(f"{TORCH_LIB_PATH} not found: build the HIP extension first "
+                               "(python -c 'import __graft_entry__ as g; g.build()'); there is no CPU fallback")
+        spec = importlib.util.spec_from_file_location("ppv_torch", TORCH_LIB_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind([(n, ctypes.cast(getattr(L, n), _P).value) for n in _TORCH_ENTRIES])
+        _torch_ops = mod
+    return _torch_ops
+
+
 def check(status, what):
     if status != 0:
         raise RuntimeError(f"libppv_hip: {what} failed with status {status}")
@@ -269,15 +291,6 @@ def stream_ptr():
     if _raw_stream is not None and _cur_device is not None:
         return ctypes.c_void_p(_raw_stream(_cur_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-_same_device = contextlib.nullcontext()
-
-
-def device_of(t):
-    """Context in which ``t``'s device is the current one (``stream_ptr`` and every launch go to the current device)."""
-    i = t.device.index
-    return _same_device if i is None or i == (_cur_device() if _cur_device is not None else torch.cuda.current_device()) else torch.cuda.device(i)
 
 
 def ptr(t):

@@ -229,62 +229,7 @@ def instance_norm_act(x, scale, shift, slope=1.0, eps=1e-5):
     return _InstNormAct.apply(x, scale, shift, float(slope), float(eps))
 
 
-ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # the dtype codes of the C ABI
-
-
-def _rows(t, C):
-    """t [..., C] as a [rows, C] view (a copy where there is none) with unit column stride."""
-    t = t.reshape(-1, C)
-    return t if t.stride(1) == 1 or C == 1 else t.contiguous()
-
-
-def _layer_norm_fwd(x2, weight, bias, eps, keep):
-    rows, C = x2.shape
-    y = torch.empty((rows, C), dtype=x2.dtype, device=x2.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x2.device) if keep else None
-    if rows:
-        par = weight if weight is not None else bias
-        with _lib.device_of(x2):
-            check(_lib.lib().ppv_layernorm_fwd(ptr(x2), x2.stride(0), ptr(weight), ptr(bias), ptr(y), stats.data_ptr() if keep else None,
-                                               stats.data_ptr() + 4 * rows if keep else None, rows, C, ELEM_TYPES[x2.dtype],
-                                               0 if par is None else ELEM_TYPES[par.dtype], eps, stream_ptr()), "ppv_layernorm_fwd")
-    return y, stats
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        x2 = _rows(x, x.shape[-1])
-        w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-        y, stats = _layer_norm_fwd(x2, w, b, eps, True)
-        ctx.save_for_backward(x2, w, stats)
-        ctx.par = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y.view(x.shape)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        x2, w, stats = ctx.saved_tensors
-        rows, C = x2.shape
-        g2 = _rows(g, C)
-        dx = torch.empty((rows, C), dtype=x2.dtype, device=x2.device)
-        wdt, bdt = ctx.par
-        dw = torch.empty(C, dtype=wdt, device=x2.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(C, dtype=bdt, device=x2.device) if ctx.needs_input_grad[2] else None
-        if rows:
-            L, code = _lib.lib(), ELEM_TYPES[x2.dtype]
-            ws = None
-            if dw is not None or db is not None:
-                ws = torch.empty(int(L.ppv_layernorm_bwd_workspace_bytes(rows, C, code)), dtype=torch.uint8, device=x2.device)
-            with _lib.device_of(x2):
-                check(L.ppv_layernorm_bwd(ptr(g2), g2.stride(0), ptr(x2), x2.stride(0), ptr(w), stats.data_ptr(), stats.data_ptr() + 4 * rows,
-                                          ptr(dx), ptr(dw), ptr(db), ptr(ws), rows, C, code, ELEM_TYPES.get(wdt or bdt, 0), stream_ptr()),
-                      "ppv_layernorm_bwd")
-        else:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        return (dx.view(g.shape) if ctx.needs_input_grad[0] else None), dw, db, None
+ELEM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -307,10 +252,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if not eps >= 0:
         raise ValueError("layer_norm: eps >= 0")
     _lib.require_cuda(x)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
-    w, b = (None if t is None else t.detach().contiguous() for t in (weight, bias))
-    return _layer_norm_fwd(_rows(x.detach(), x.shape[-1]), w, b, float(eps), False)[0].view(x.shape)
+    return _lib.torch_ops().layer_norm(x, weight, bias, eps)
 
 
 # ------------------------------------------------------------------------------------------------------------------------------------

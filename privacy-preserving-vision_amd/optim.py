@@ -7,6 +7,7 @@ encoder.parameters()), lr=encoder_lr)`` and the decoder's twin), stepped at ``tr
 ``amsgrad``, ``maximize``, ``capturable``, sparse or non-f32 gradients.  No CPU / stock-torch fallback: the HIP library does the step.
 
 ``ppv_amd.optim.AdamW``: torch.optim.AdamW (decoupled weight decay) the same way, with its moments in 32 or in 8 bits (``csrc/adamw.hip``)."""
+import operator
 import struct
 
 import numpy as np
@@ -124,7 +125,7 @@ class AdamW(torch.optim.Optimizer):
         if min_8bit_size < 0:
             raise ValueError("ppv_amd.optim.AdamW: min_8bit_size >= 0")
         self.state_bits, self.min_8bit_size, self.seed = state_bits, min_8bit_size, int(seed)
-        self._tables = {}                      # (group index, slot) -> (the addresses it holds, descriptor table on the device, its blocks)
+        self._tables = {}                       # (group index, slot) -> (parameters, their moments, the native list of both)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
                                       foreach=None, capturable=False, differentiable=False, fused=None))
 
@@ -175,35 +176,21 @@ class AdamW(torch.optim.Optimizer):
             return st["exp_avg"], st["exp_avg_sq_root"], st["exp_avg_scale"], st["exp_avg_sq_root_scale"]
         return st["exp_avg"], st["exp_avg_sq"], None, None
 
-    def _table(self, slot, ps):
-        moments = [self._moments(self.state[p]) for p in ps]
-        # every address that the records hold is in the key (and the stream that the table was written on): another one, another table
-        key = [p.data_ptr() for p in ps] + [p.grad.data_ptr() for p in ps] + [t.data_ptr() for m in moments for t in m if t is not None]
-        key.append(_lib.stream_ptr().value)
+    def _list(self, slot, ps):
+        """The native list of these parameters with their moments; kept while both are the same tensors."""
+        sts = [self.state[p] for p in ps]
+        held = [t for st in sts for t in self._moments(st)]
         hit = self._tables.get(slot)
-        if hit is not None and hit[0] == key:
-            return hit[1], hit[2], hit[3]
-        recs, blk = [], 0
-        for p, (m, v, ms, vs) in zip(ps, moments):
-            n = p.numel()
-            if n == 0:
-                continue
-            ok = all(t.device == p.device and t.is_contiguous() and t.numel() == n for t in (m, v))
-            if ms is None:
-                ok = ok and m.dtype == v.dtype == torch.float32
-            else:
-                ok = ok and m.dtype == v.dtype == torch.float8_e4m3fn and all(
-                    t.device == p.device and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == (n + 255) // 256 for t in (ms, vs))
-            if not ok:
+        if hit is not None and len(hit[0]) == len(ps) and all(map(operator.is_, hit[0], ps)) and all(map(operator.is_, hit[1], held)):
+            return hit[2]
+        for p, (m, v, ms, vs) in zip(ps, zip(*[iter(held)] * 4)):
+            n, kind = p.numel(), torch.float32 if ms is None else torch.float8_e4m3fn
+            if not (all(t.device == p.device and t.is_contiguous() and t.numel() == n and t.dtype == kind for t in (m, v)) and (ms is None or all(
+                    t.device == p.device and t.is_contiguous() and t.numel() == (n + 255) // 256 and t.dtype == torch.float32 for t in (ms, vs)))):
                 raise ValueError("ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)")
-            recs.append(struct.pack("<QQQQQQqiI", p.data_ptr(), p.grad.data_ptr(), m.data_ptr(), v.data_ptr(), ms.data_ptr() if ms is not None else 0,
-                                    vs.data_ptr() if vs is not None else 0, n, blk, self._place[p] & 0xFFFFFFFF))
-            blk += (n + _CHUNK - 1) // _CHUNK
-        desc = None
-        if recs:                               # pinned and non-blocking: a list whose gradients move every step does not wait for the device
-            desc = torch.frombuffer(bytearray(b"".join(recs)), dtype=torch.uint8).pin_memory().to(ps[0].device, non_blocking=True)
-        self._tables[slot] = (key, desc, len(recs), blk)
-        return desc, len(recs), blk
+        native = _lib.torch_ops().AdamWList(ps, held[0::4], held[1::4], held[2::4], held[3::4], [self._place[p] & 0xFFFFFFFF for p in ps])
+        self._tables[slot] = (ps, held, native)
+        return native
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -211,34 +198,25 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        L = _lib.lib()
-        f32, strided = torch.float32, torch.strided
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
                 continue
-            dev = ps[0].device
+            if ps[0].device.type != "cuda":
+                raise NotImplementedError("ppv_amd.optim.AdamW: contiguous f32 parameters and gradients on one GPU only")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("ppv_amd.optim.AdamW: a step cannot be captured into a graph (its number is part of the launch)")
             for p in ps:
-                g = p.grad
-                if (g.dtype is not f32 or p.dtype is not f32 or g.layout is not strided or not g.is_contiguous() or not p.is_contiguous()
-                        or p.device != dev or g.device != dev or g.numel() != p.numel() or dev.type != "cuda"):
-                    raise NotImplementedError("ppv_amd.optim.AdamW: contiguous f32 parameters and gradients on one GPU only")
                 if not self.state[p]:
                     self._init_state(p)
-            with _lib.device_of(ps[0]):
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("ppv_amd.optim.AdamW: a step cannot be captured into a graph (its number is part of the launch)")
-                by_step = {}                   # parameters whose gradient was missing in some step keep their own count
-                for p in ps:
-                    by_step.setdefault(float(self.state[p]["step"]), []).append(p)
-                for k in [k for k in self._tables if k[0] == gi and k[1] >= len(by_step)]:
-                    del self._tables[k]
-                b1, b2 = group["betas"]
-                for slot, (t, sub) in enumerate(sorted(by_step.items())):
-                    desc, n, blocks = self._table((gi, slot), sub)
-                    if n:
-                        _lib.check(L.ppv_adamw_multi(desc.data_ptr(), n, blocks, float(group["lr"]), b1, b2, group["eps"], group["weight_decay"],
-                                                     t + 1.0, self.seed & 0xFFFFFFFF, _lib.stream_ptr()), "ppv_adamw_multi")
-                    for p in sub:
-                        self.state[p]["step"] = t + 1.0
+            by_step = {}                       # parameters whose gradient was missing in some step keep their own count
+            for p in ps:
+                by_step.setdefault(float(self.state[p]["step"]), []).append(p)
+            for k in [k for k in self._tables if k[0] == gi and k[1] >= len(by_step)]:
+                del self._tables[k]
+            b1, b2 = group["betas"]
+            for slot, (t, sub) in enumerate(sorted(by_step.items())):
+                self._list((gi, slot), sub).step(group["lr"], b1, b2, group["eps"], group["weight_decay"], t + 1.0, self.seed & 0xFFFFFFFF)
+                for p in sub:
+                    self.state[p]["step"] = t + 1.0
         return loss

@@ -314,3 +314,20 @@ def test_attention_entry_points_refuse():
     for kw in ({"sgt": 12}, {"dout": 72}, {"dk": 8}):
         assert L.ppv_attention_bwd(args(**kw), None) == SIZE, kw
     assert L.ppv_attention_fwd_workspace_bytes(1, 3, 2, 1, 1, 8, 1) == 0 and L.ppv_attention_bwd_workspace_bytes(0, 1, 1) == 0
+
+
+@pytest.mark.gpu
+def test_attention_is_differentiable_once_and_keeps_what_it_needs():
+    from ppv_amd.attention import multihead_attention
+    q, k, v, g = (t.cuda() for t in _inputs(1, 5, 9, 2, 2, 16, torch.float32, 1))
+    q.requires_grad_(True)
+    want, = torch.autograd.grad(multihead_attention(q, k, v), q, g)
+    dq, = torch.autograd.grad(multihead_attention(q, k, v), q, g, create_graph=True)
+    assert torch.equal(dq, want)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dq.sum().backward()
+    lens = torch.tensor([4], dtype=torch.int32, device="cuda")
+    out = multihead_attention(q, k, v, k_lens=lens)
+    lens.fill_(9)                                                  # lengths are operands: changed under a pending backward pass, they are refused
+    with pytest.raises(RuntimeError):
+        out.sum().backward()

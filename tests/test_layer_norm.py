@@ -216,3 +216,16 @@ def test_layer_norm_entry_points_refuse():
     assert L.ppv_layernorm_bwd(p, 8, p, 8, p, p, p, p, p, p, p, 1, 8, 0, 5, None) == SIZE
     assert L.ppv_layernorm_bwd_workspace_bytes(0, 8, 0) == 0
     assert L.ppv_layernorm_bwd_workspace_bytes(10, 8, 0) >= 2 * 8 * 4
+
+
+@pytest.mark.gpu
+def test_layer_norm_is_differentiable_once():
+    """A graph of the backward pass can be asked for; differentiating through it is an error, not a silent zero."""
+    from ppv_amd.nn_ops import layer_norm
+    x, w, b, dy = (t.cuda() for t in _case(6, 40, torch.float32, torch.float32, 4))
+    x.requires_grad_(True)
+    want, = torch.autograd.grad(layer_norm(x, w, b), x, dy)
+    dx, = torch.autograd.grad(layer_norm(x, w, b), x, dy, create_graph=True)
+    assert torch.equal(dx, want)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dx.sum().backward()
