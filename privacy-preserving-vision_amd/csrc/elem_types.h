@@ -53,6 +53,19 @@ template <class T> __device__ __forceinline__ u32x4 pack_vec(const float (&v)[16
     return r;
 }
 
+// the 16 bytes at p as they are (any alignment of T); elements at or behind `left` are zeros and are not touched
+template <class T> __device__ __forceinline__ u32x4 load_raw(const T* p, int left) {
+    constexpr int V = 16 / sizeof(T);
+    if (left >= V) return *reinterpret_cast<const typename Raw16<T>::type*>(p);
+    u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < left) {
+            if constexpr (sizeof(T) == 4) r[e] = *reinterpret_cast<const unsigned*>(p + e);
+            else r[e / 2] |= (unsigned)p[e].u << (16 * (e & 1));
+        }
+    return r;
+}
 // the 16 / sizeof(T) elements at p (any alignment of T); those at or behind `left` read as zero and are not touched
 template <class T, int V> __device__ __forceinline__ void load_vec(const T* p, int left, float (&o)[V]) {
     if (left >= V) {

@@ -7,8 +7,11 @@
 // (16, a wave, or a workgroup), NV 16-byte vectors each, so the variance is the two-pass one (sum of squared distances from the mean: no
 // cancellation for rows far from zero) without reading the row again.  All sums are f32.  Rows may start at any element: the 16-byte
 // loads ask for element alignment only (global memory takes them), the last vector of a row is taken element by element.
-// Backward: a fixed grid strides over the rows, every lane keeps the weight-gradient sums of its columns in registers, a workgroup
-// leaves one partial row, a second launch adds the partial rows in their order (no atomics: the same bits every time).
+// Backward: a fixed grid strides over the rows, the next row's operands are on their way while one is worked on, every lane keeps the
+// weight-gradient sums of its columns in registers, a workgroup leaves one partial row, a second launch adds the partial rows in their order (no atomics:
+// the same bits every time).
+// Measured (MI355X): 165888 rows of 2048 bf16, forward 245 us = 5.5 TB/s, backward 370 us = 5.5 TB/s (without the next row's loads, 32
+// elements a lane: 560); 6656 rows of 512: 5 + 11 + 4 us, less than the host takes to ask for them.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include "ppv_common.h"
@@ -122,15 +125,50 @@ __global__ __launch_bounds__(256) void layernorm_fwd_long_kernel(const T* __rest
     if (mean_out && threadIdx.x == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
 }
 
+// two sums at once over the LPR lanes of a row's group
+template <int LPR> __device__ __forceinline__ void group_sum2(float& a, float& b, float (*lds)[2]) {
+    a = row16_sum_f(a);
+    b = row16_sum_f(b);
+    if constexpr (LPR >= 64) { a = wave_sum_of_rows(a); b = wave_sum_of_rows(b); }
+    if constexpr (LPR > 64) {
+        constexpr int NW = LPR / 64;
+        if ((threadIdx.x & 63) == 0) { lds[threadIdx.x >> 6][0] = a; lds[threadIdx.x >> 6][1] = b; }
+        __syncthreads();
+        const int w0 = threadIdx.x / LPR * NW;
+        a = lds[w0][0];
+        b = lds[w0][1];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) { a += lds[w0 + i][0]; b += lds[w0 + i][1]; }
+        __syncthreads();
+    }
+}
+
 template <class T, int LPR, int NV, int NT>
-__global__ __launch_bounds__(NT) void layernorm_bwd_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
-                                                           const void* __restrict__ w, int wdtype, const float* __restrict__ mean_in,
-                                                           const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
-                                                           long rows, int C) {
+__global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
+                                                              const void* __restrict__ w, int wdtype, const float* __restrict__ mean_in,
+                                                              const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ part,
+                                                              long rows, int C) {
     constexpr int V = 16 / sizeof(T), RPW = NT / LPR;
-    extern __shared__ float smem[];                            // [2][C] partial sums (LPR <= 64), then the words of group_sum
-    __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
+    extern __shared__ float smem[];                            // LPR < NT: the waves' (row slots') sums, [C] each
+    __shared__ float lds[LPR > 64 ? NT / 64 : 1][2];
     const int l = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    const float inv_c = 1.f / (float)C;
+    const long step = (long)gridDim.x * RPW, turns = (rows + step - 1) / step, row0 = (long)blockIdx.x * RPW + grp;
+    u32x4 gr[NV], xr[NV];
+    float mean, rstd;
+    auto fetch = [&](long row) {
+        const bool live = row < rows;
+        const long at = live ? row : 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            gr[i] = load_raw<T>(g + at * ldg + c, live ? C - c : 0);
+            xr[i] = load_raw<T>(x + at * ldx + c, live ? C - c : 0);
+        }
+        mean = mean_in[at];
+        rstd = rstd_in[at];
+    };
+    fetch(row0);
     float wv[NV][V], aw[NV][V], ab[NV][V];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -139,27 +177,25 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_kernel(const T* __restrict__
 #pragma unroll
         for (int e = 0; e < V; ++e) aw[i][e] = ab[i][e] = 0.f;
     }
-    const float inv_c = 1.f / (float)C;
-    const long step = (long)gridDim.x * RPW, turns = (rows + step - 1) / step;
     for (long t = 0; t < turns; ++t) {                         // the same number of turns for every lane: the sums cross lanes and waves
-        const long row = t * step + (long)blockIdx.x * RPW + grp;
+        const long row = t * step + row0;
         const bool live = row < rows;
-        const long at = live ? row : 0;
         float gv[NV][V], hv[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * LPR + l) * V;
-            load_vec<T, V>(g + at * ldg + c, live ? C - c : 0, gv[i]);
-            load_vec<T, V>(x + at * ldx + c, live ? C - c : 0, hv[i]);
+            unpack_vec<T>(gr[i], gv[i]);
+            unpack_vec<T>(xr[i], hv[i]);
         }
-        const float mean = mean_in[at], rstd = rstd_in[at];
+        const float mu = mean, rs = rstd;
+        if (t + 1 < turns) fetch(row + step);                  // the next row comes while this one is worked on
+        __builtin_amdgcn_sched_barrier(0);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int left = live ? C - (i * LPR + l) * V : 0;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float h = e < left ? (hv[i][e] - mean) * rstd : 0.f, gw = gv[i][e] * wv[i][e];   // (g is zero behind the row)
+                const float h = e < left ? (hv[i][e] - mu) * rs : 0.f, gw = gv[i][e] * wv[i][e];       // (g is zero behind the row)
                 aw[i][e] = __builtin_fmaf(gv[i][e], h, aw[i][e]);
                 ab[i][e] += gv[i][e];
                 s1 += gw;
@@ -168,8 +204,9 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_kernel(const T* __restrict__
                 gv[i][e] = gw;
             }
         }
-        s1 = group_sum<LPR>(s1, lds) * inv_c;
-        s2 = group_sum<LPR>(s2, lds) * inv_c;
+        group_sum2<LPR>(s1, s2, lds);
+        s1 *= inv_c;
+        s2 *= inv_c;
         if (!live) continue;
         T* dr = dx + row * (long)C;
 #pragma unroll
@@ -178,35 +215,41 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_kernel(const T* __restrict__
             if (c >= C) continue;
             float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = rstd * (gv[i][e] - s1 - hv[i][e] * s2);
+            for (int e = 0; e < V; ++e) o[e] = rs * (gv[i][e] - s1 - hv[i][e] * s2);
             store_vec<T, V>(dr + c, C - c, o);
         }
     }
     if (!part) return;
     float* pw = part + (long)blockIdx.x * 2 * C;
-    if constexpr (LPR <= 64) {                                 // several rows at a time in this workgroup: their sums meet in LDS, in order
+    if constexpr (LPR < NT) {                                  // several rows at a time in this workgroup: their sums meet in LDS, added in order
         if constexpr (LPR < 64) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int e = 0; e < V; ++e) { aw[i][e] = wave_sum_of_rows(aw[i][e]); ab[i][e] = wave_sum_of_rows(ab[i][e]); }
         }
-        for (int wv_ = 0; wv_ < NT / 64; ++wv_) {
-            if ((int)(threadIdx.x >> 6) == wv_ && (threadIdx.x & 63) < LPR) {
+        constexpr int PARTS = LPR <= 64 ? NT / 64 : RPW;
+        const int part_of = LPR <= 64 ? threadIdx.x >> 6 : grp;
+        auto meet = [&](float (&v)[NV][V], float* out) {
+            if (LPR >= 64 || (threadIdx.x & 63) < LPR)
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         const int c = (i * LPR + l) * V + e;
-                        if (c < C) {
-                            smem[c] = wv_ ? smem[c] + aw[i][e] : aw[i][e];
-                            smem[C + c] = wv_ ? smem[C + c] + ab[i][e] : ab[i][e];
-                        }
+                        if (c < C) smem[part_of * C + c] = v[i][e];
                     }
-            }
             __syncthreads();
-        }
-        for (int c = threadIdx.x; c < 2 * C; c += NT) pw[c] = smem[c];
+            for (int c = threadIdx.x; c < C; c += NT) {
+                float s = smem[c];
+#pragma unroll
+                for (int k = 1; k < PARTS; ++k) s += smem[k * C + c];
+                out[c] = s;
+            }
+        };
+        meet(aw, pw);
+        __syncthreads();
+        meet(ab, pw + C);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -287,20 +330,22 @@ __global__ __launch_bounds__(256) void layernorm_wgrad_reduce_kernel(const float
     }
 }
 
-// workgroups of the backward pass: enough to fill the chip, at least four rows for each row slot, so that the partial rows stay few
+// workgroups of the backward pass: two for each CU (165888 rows of 2048 bf16: 512 and 256 take 620 us with the forward pass, 768 650, 1024 690,
+// 2048 710: more streams at once are worse for the memory), at least four rows for each row slot, so that the partial rows stay few
 static int layernorm_bwd_groups(long rows, int C, int rpw) {
     const long by_rows = (rows + 4L * rpw - 1) / (4L * rpw);
-    const long most = C > 16384 ? 64 : 512;
+    const long most = C > 8192 ? 64 : 512;
     return (int)(by_rows < 1 ? 1 : by_rows > most ? most : by_rows);
 }
-// vectors of a row -> lanes per row of the backward kernels (at most 32 elements a lane: two gradient sums, a weight and two operands each)
+// lanes per row of the backward kernels: at most 16 elements a lane (two gradient sums, a weight and two operands each; with 32 the next row's
+// loads no longer fit beside them), 0: longer than the registers hold
 static int layernorm_bwd_lpr(int C, int dtype) {
-    const int v = dtype == 0 ? 4 : 8, nvec = (C + v - 1) / v, most = 32 / v;
-    return nvec <= 16 ? 16 : nvec <= 64 * most ? 64 : nvec <= 256 * most ? 256 : nvec <= 512 * most ? 512 : 0;
+    const int v = dtype == 0 ? 4 : 8, nvec = (C + v - 1) / v, most = 16 / v;
+    return nvec <= 16 ? 16 : nvec <= 64 * most ? 64 : nvec <= 128 * most ? 128 : nvec <= 256 * most ? 256 : nvec <= 512 * most ? 512 : 0;
 }
 static int layernorm_groups_of(long rows, int C, int dtype) {
     const int lpr = layernorm_bwd_lpr(C, dtype);
-    return layernorm_bwd_groups(rows, C, lpr == 16 ? 16 : lpr == 64 ? 4 : 1);
+    return layernorm_bwd_groups(rows, C, lpr == 0 || lpr >= 256 ? 1 : 256 / lpr);
 }
 
 template <class T>
@@ -330,19 +375,16 @@ static int layernorm_bwd_t(const T* g, long ldg, const T* x, long ldx, const voi
     constexpr int V = 16 / sizeof(T);
     const int nvec = (C + V - 1) / V, lpr = layernorm_bwd_lpr(C, dtype), G = layernorm_groups_of(rows, C, dtype);
     if (!dw && !db) part = nullptr;
-#define LN_BWD(LPR, NV, NT) \
-    layernorm_bwd_kernel<T, LPR, NV, NT><<<G, NT, LPR <= 64 ? 2 * C * sizeof(float) : 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, part, rows, C)
+#define LN_BWD(LPR, NV, NT)                                                                                                              \
+    layernorm_bwd_kernel<T, LPR, NV, NT><<<G, NT, (LPR >= NT ? 0 : LPR <= 64 ? NT / 64 : NT / LPR) * C * sizeof(float), stream>>>(        \
+        g, ldg, x, ldx, w, wdtype, mean, rstd, dx, part, rows, C)
     if (lpr == 16) LN_BWD(16, 1, 256);
-    else if (lpr == 64) {
-        if (nvec <= 64) LN_BWD(64, 1, 256);
-        else if (nvec <= 128) LN_BWD(64, 2, 256);
-        else if (nvec <= 256) LN_BWD(64, 4, 256);
-        else LN_BWD(64, 32 / V, 256);                          // (f32 only: 8 vectors; the 16-bit types end at 4)
-    } else if (lpr == 256) {
-        if (nvec <= 512) LN_BWD(256, 2, 256);
-        else if (nvec <= 1024) LN_BWD(256, 4, 256);
-        else LN_BWD(256, 32 / V, 256);
-    } else if (lpr == 512) LN_BWD(512, 32 / V, 512);
+    else if (lpr == 64 && nvec <= 64) LN_BWD(64, 1, 256);
+    else if (lpr == 64 && nvec <= 128) LN_BWD(64, 2, 256);
+    else if (lpr == 64) LN_BWD(64, 16 / V, 256);               // (f32: 4 vectors; the 16-bit types end at 2)
+    else if (lpr == 128) LN_BWD(128, 16 / V, 256);
+    else if (lpr == 256) LN_BWD(256, 16 / V, 256);
+    else if (lpr == 512) LN_BWD(512, 16 / V, 512);
     else {
         if (rows > 0x7fffffffL) return PPV_ERR_BAD_SIZE;
         layernorm_bwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, C);

@@ -23,8 +23,8 @@ def _case(rows, cols, dt, wdt, seed, offset=1.0):
 
 
 def _check(x, w, b, dy, y, dx, dw, db, eps):
-    """Bounds by counting roundings: a sum over a row is at most 32 additions in a lane and 10 across lanes (rows that are longer than the
-    registers: C / 1024 in a lane), a row's mean is off by at most K u max|x| with K = 48 + C / 1024, and so is x - mean; h = (x - mean) rstd
+    """Bounds by counting roundings: a sum over a row is at most 32 additions in a lane and 16 across lanes (rows that are longer than the
+    registers: C / 256 in a lane), a row's mean is off by at most K u max|x| with K = 48 + C / 256, and so is x - mean; h = (x - mean) rstd
     is off by E = K u max|x| rstd plus 3 u |h|, and rstd's own error is of the same order.  Each result is rounded once to its type."""
     rows, C = x.shape
     dt, wdt = y.dtype, (w.dtype if w is not None else torch.float32)
@@ -34,7 +34,7 @@ def _check(x, w, b, dy, y, dx, dw, db, eps):
     ref = orc.layer_norm(xd, wd, bd, eps)
     gx, gw, gb = torch.autograd.grad(ref, (xd, wd, bd), dyd)
     xd, ref, wd = xd.detach(), ref.detach(), wd.detach()
-    K = 48 + C / 1024
+    K = 48 + C / 256
     rstd = 1 / torch.sqrt(xd.var(1, unbiased=False, keepdim=True) + eps)
     h = (xd - xd.mean(1, keepdim=True)) * rstd
     E = K * U * (xd.abs().amax(1, keepdim=True) * rstd + h.abs()) + K * U * h.abs().amax(1, keepdim=True)
