@@ -1,7 +1,7 @@
 // Multi-head attention, forward (gfx950):  S = scale Q K^T,  P = softmax over the visible keys,  O = P V,  and log-sum-exp for the backward pass.
 //
-// One pass over the keys with a running maximum m and sum l (in units of log2): a tile's P is exp2(S c - m), the accumulated O and l are
-// scaled by exp2(m_old - m_new).  Neither S nor P reaches memory.  Training and prefill are bound by the matrix pipe and the exponentials,
+// One pass over the keys with a running maximum m and sum l (in units of log2): a tile's P is exp2(S c - m); where m grows, the accumulated O and
+// l are scaled by exp2(m_old - m_new).  Neither S nor P reaches memory.  Training and prefill are bound by the matrix pipe and the exponentials,
 // a few rows against a long history by the bytes of K and V.
 //   * a wave owns 32 rows as the columns of S^T = K Q^T and O^T = V^T P^T (attention_tiles.h): m, l and the scaling are one scalar per
 //     lane, P goes from accumulator to operand in place;
@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
         for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     float m = -__builtin_inff(), l = 0.f;
     const float c = d.scale * LOG2E;
+    const auto L = TL::lane_part(lane);
 
     for (int kt = kt0, buf = 0; kt < kt1; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
@@ -144,9 +145,9 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[mb][j] = 0.f;
 #pragma unroll
-            for (int kd = 0; kd < TL::NF; ++kd) s[mb] = TL::mma(TL::by_row(tk, own + mb * 32, kd, lane), qf[kd], s[mb]);
+            for (int kd = 0; kd < TL::NF; ++kd) s[mb] = TL::mma(TL::by_row(tk, L, own + mb * 32, kd), qf[kd], s[mb]);
         }
-        if (kt * KT + KT - 1 > lim0) {                         // a key of this tile is hidden from some row
+        if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
 #pragma unroll
             for (int mb = 0; mb < MBW; ++mb)
 #pragma unroll
@@ -159,9 +160,18 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, s[mb][j]);
         top = half_swap_max(top) * c;
-        const float mn = fmaxf(m, top), mu = mn == -__builtin_inff() ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - mu);
-        m = mn;
+        // The running maximum follows only where it has grown by more than 2^8 (P, l and O then stay below 256 times what they would be: nothing
+        // to f32, and P's rounding is relative).  Without the hint the branch becomes 64 products and 64 copies in every tile.
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0, 0)) {
+            const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(mn == -__builtin_inff() ? 0.f : m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
+        }
+        const float mu = m == -__builtin_inff() ? 0.f : m;
         float sum = 0.f;
 #pragma unroll
         for (int mb = 0; mb < MBW; ++mb)
@@ -170,20 +180,14 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
                 s[mb][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mb][j], c, -mu));
                 sum += s[mb][j];
             }
-        l = __builtin_fmaf(l, alpha, sum);
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < TL::DB; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[i][j] *= alpha;
-        }
+        l += sum;
 #pragma unroll
         for (int mb = 0; mb < MBW; ++mb)
 #pragma unroll
             for (int kf = 0; kf < TL::CF; ++kf) {
                 const u32x4 pf = TL::from_acc(s[mb], kf);
 #pragma unroll
-                for (int i = 0; i < TL::DB; ++i) o[i] = TL::mma(TL::by_col(tv, own + mb * 32, i, kf, lane), pf, o[i]);
+                for (int i = 0; i < TL::DB; ++i) o[i] = TL::mma(TL::by_col(tv, L, own + mb * 32, i, kf), pf, o[i]);
             }
     }
     l = half_swap_sum(l);

@@ -28,7 +28,7 @@ template <class T, int DP, int OG, int ACC> struct BwdShape {
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
-    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG == 1 || ACC == 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
+    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG < ACC * 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
 };
 // adds the other groups' accumulators to the first one's (in their order); false: this wave is done
 template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* acc, float* lds, int og, int sg, int lane) {
@@ -122,6 +122,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
 
+    const auto L = TL::lane_part(lane);
     const int own = sg * 32;                                   // this group's rows of a tile
     for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
@@ -138,21 +139,21 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
         for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
-            s = TL::mma(TL::by_row(tk, own, kd, lane), qf[kd], s);
-            p = TL::mma(TL::by_row(tv, own, kd, lane), gf[kd], p);
+            s = TL::mma(TL::by_row(tk, L, own, kd), qf[kd], s);
+            p = TL::mma(TL::by_row(tv, L, own, kd), gf[kd], p);
         }
-        const bool hidden = kt * KT + KT - 1 > lim0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * (p[j] - delta);
-            if (hidden && kt * KT + own + 8 * (j >> 2) + 4 * half + (j & 3) > lim) ds = 0.f;
-            s[j] = ds;
+        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * (p[j] - delta);
+        if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (kt * KT + own + 8 * (j >> 2) + 4 * half + (j & 3) > lim) s[j] = 0.f;
         }
 #pragma unroll
         for (int kf = 0; kf < TL::CF; ++kf) {
             const u32x4 df = TL::from_acc(s, kf);
 #pragma unroll
-            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, own, i, kf, lane), df, acc[i]);
+            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, L, own, i, kf), df, acc[i]);
         }
     }
     if (SG > 1) __syncthreads();
@@ -177,7 +178,11 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     using TL = Tile<T, DP>;
     using SH = BwdShape<T, DP, OG, 1>;                         // (dK and dV meet one after the other)
     constexpr int NT = 256, QT = SH::KT, NB = SH::NB, SG = SH::SG;
+    // K, V, dK, dV of 128 in registers leave one wave per SIMD (328 registers: 580 us where this form takes 390, 2 x 16 heads of 4096
+    // tokens, causal): V waits in LDS instead
+    constexpr bool VL = DP == 128 && sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
+    __shared__ __attribute__((aligned(16))) char vown[VL ? TL::bytes(OG * 32) : 16];
     __shared__ __attribute__((aligned(16))) float stat[NB][2][QT];     // lse, delta
     __shared__ __attribute__((aligned(16))) int limit[NB][QT];         // last key that a row sees
     const AttnDims& d = a.d;
@@ -219,9 +224,13 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         }
     };
     if (rt0 < rt1) fetch(rt0);
-    u32x4 kf_[TL::NF], vf[TL::NF];
+    u32x4 kf_[TL::NF], vf[VL ? 1 : TL::NF];
     load_own<T, DP>(kf_, K, key, klen, nch, lane);
-    load_own<T, DP>(vf, V, key, klen, nch, lane);
+    if constexpr (VL) {
+        Stager<T, DP, OG * 32, NT> sv;
+        sv.fetch(V, key0, klen, nch, tid);
+        sv.put(vown, tid);                                     // (the first tile's barrier comes before its first reader)
+    } else load_own<T, DP>(vf, V, key, klen, nch, lane);
     const float c = d.scale * LOG2E;
     f32x16 dk[TL::DB], dv[TL::DB];
 #pragma unroll
@@ -229,6 +238,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
 #pragma unroll
         for (int j = 0; j < 16; ++j) dk[i][j] = dv[i][j] = 0.f;
 
+    const auto L0 = TL::lane_part(lane);
     const int own = sg * 32;
     for (int rt = rt0, buf = 0; rt < rt1; ++rt, buf ^= NB - 1) {
         char *tq = smem + buf * 2 * TL::bytes(QT), *tg = tq + TL::bytes(QT);
@@ -241,28 +251,41 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         }
         __syncthreads();
         if (rt + 1 < rt1) fetch(rt + 1);
+        // (opaque in each turn: the 16 addresses made from it are then computed where they are used and not kept in 16 registers)
+        auto L = L0;
+        asm volatile("" : "+v"(L.row), "+v"(L.col0), "+v"(L.col1));
         f32x16 s, p;
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
         for (int kd = 0; kd < TL::NF; ++kd) {
-            s = TL::mma(TL::by_row(tq, own, kd, lane), kf_[kd], s);
-            p = TL::mma(TL::by_row(tg, own, kd, lane), vf[kd], p);
+            s = TL::mma(TL::by_row(tq, L, own, kd), kf_[kd], s);
+            if constexpr (VL) p = TL::mma(TL::by_row(tg, L, own, kd), TL::by_row(vown, L, og * 32, kd), p);
+            else p = TL::mma(TL::by_row(tg, L, own, kd), vf[kd], p);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int r = own + 8 * g + 4 * half;
             const float4 ls = *reinterpret_cast<const float4*>(&stat[buf][0][r]), de = *reinterpret_cast<const float4*>(&stat[buf][1][r]);
-            const int4 li = *reinterpret_cast<const int4*>(&limit[buf][r]);
             const float lsv[4] = {ls.x, ls.y, ls.z, ls.w}, dev[4] = {de.x, de.y, de.z, de.w};
-            const int liv[4] = {li.x, li.y, li.z, li.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = 4 * g + i;
-                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lsv[i])), ds = pe * (p[j] - dev[i]);
-                const bool seen = key <= liv[i];
-                p[j] = seen ? pe : 0.f;
-                s[j] = seen ? ds : 0.f;
+                const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lsv[i]));
+                s[j] = pe * (p[j] - dev[i]);
+                p[j] = pe;
+            }
+        }
+        // a key of this workgroup is hidden from some row of the tile, or the tile is not full
+        const int t0 = (int)((unsigned)(rt * QT) / (unsigned)d.G), lim0 = d.causal ? min(klen - 1, t0 + shift) : klen - 1;
+        if (__builtin_expect(key0 + OG * 32 - 1 > lim0 || (rt + 1) * QT > rows, 0)) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int4 li = *reinterpret_cast<const int4*>(&limit[buf][own + 8 * g + 4 * half]);
+                const int liv[4] = {li.x, li.y, li.z, li.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key > liv[i]) p[4 * g + i] = s[4 * g + i] = 0.f;
             }
         }
 #pragma unroll
@@ -270,8 +293,8 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             const u32x4 pf = TL::from_acc(p, kf), df = TL::from_acc(s, kf);
 #pragma unroll
             for (int i = 0; i < TL::DB; ++i) {
-                dv[i] = TL::mma(TL::by_col(tg, own, i, kf, lane), pf, dv[i]);
-                dk[i] = TL::mma(TL::by_col(tq, own, i, kf, lane), df, dk[i]);
+                dv[i] = TL::mma(TL::by_col(tg, L, own, i, kf), pf, dv[i]);
+                dk[i] = TL::mma(TL::by_col(tq, L, own, i, kf), df, dk[i]);
             }
         }
     }

@@ -50,24 +50,32 @@ template <class T, int DP> struct Tile {
         if constexpr (ES == 2) return row * ROW + ((ch ^ key(row)) << 4);
         else return row * ROW + (ch << 4);
     }
-    // A operand with m = row0 + lane % 32, k along the head dimension (fragment kd)
-    static __device__ __forceinline__ u32x4 by_row(const char* tile, int row0, int kd, int lane) {
-        return *reinterpret_cast<const u32x4*>(tile + at(row0 + (lane & 31), kd * 2 + (lane >> 5)));
+    // A lane's own part of the addresses below; what a fragment adds are constants (16-bit: XORed into the chunk bits, which no row stride reaches)
+    struct Lane { unsigned row, col0, col1; };
+    static __device__ __forceinline__ Lane lane_part(int lane) {
+        const int half = lane >> 5, r = 4 * half + ((lane >> 2) & 3), ch = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        if constexpr (ES == 2)
+            return {(unsigned)at(lane & 31, half), (unsigned)(at(r, ch) + (lane & 1) * 8), (unsigned)(at(r + 8, ch) + (lane & 1) * 8)};
+        else return {(unsigned)at(lane & 31, half), (unsigned)(4 * half * ROW + (lane & 31) * 4), 0u};
+    }
+    // A operand with m = row0 + lane % 32, k along the head dimension (fragment kd); row0 a multiple of 16
+    static __device__ __forceinline__ u32x4 by_row(const char* tile, const Lane& l, int row0, int kd) {
+        const unsigned off = ES == 2 ? l.row ^ (unsigned)(kd << 5) : l.row + (unsigned)(kd << 5);
+        return *reinterpret_cast<const u32x4*>(tile + row0 * ROW + off);
     }
     // A operand with m = 32 db + lane % 32 along the head dimension, k over the rows (fragment kf of the 32 rows from row0)
-    static __device__ __forceinline__ u32x4 by_col(const char* tile, int row0, int db, int kf, int lane) {
+    static __device__ __forceinline__ u32x4 by_col(const char* tile, const Lane& l, int row0, int db, int kf) {
         if constexpr (ES == 2) {
-            const int row = row0 + kf * 16 + 4 * (lane >> 5) + ((lane >> 2) & 3), ch = db * 4 + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
             typedef __attribute__((address_space(3))) s16x4_ lds_s16x4;
-            const s16x4_ lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + at(row, ch) + (lane & 1) * 8));
-            const s16x4_ hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + at(row + 8, ch) + (lane & 1) * 8));
+            const char* t = tile + (row0 + kf * 16) * ROW;
+            const s16x4_ lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t + (l.col0 ^ (unsigned)(db << 6))));
+            const s16x4_ hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(t + (l.col1 ^ (unsigned)(db << 6))));
             const s16x8_ v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             return __builtin_bit_cast(u32x4, v);
         } else {
-            const int row = row0 + kf * 8 + 4 * (lane >> 5);
             u32x4 v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned*>(tile + (row + j) * ROW + (db * 32 + (lane & 31)) * 4);
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const unsigned*>(tile + (row0 + kf * 8 + j) * ROW + db * 128 + l.col0);
             return v;
         }
     }
@@ -113,18 +121,14 @@ __device__ __forceinline__ int attn_len(const int* lens, int b, int most) {
     return n < 0 ? 0 : n > most ? most : n;
 }
 // blockIdx.x -> (sequence * Hkv + key head, tile).  Workgroups go round the 8 XCDs; with xcd set the tiles of one (sequence, key head) come
-// 8 apart, so that one L2 serves them.  false: past the end.
+// 8 apart, so that one L2 serves them.  Causal tiles differ in length: the first tiles of all heads come first (the caller's tile 0 is the
+// longest), then all second ones; head by head the last head's longest tile would start when the others are nearly done.  false: past the end.
 __device__ __forceinline__ bool attn_block(const AttnDims& d, int ntile, int& bh, int& tile) {
-    const int id = blockIdx.x;
-    if (d.xcd) {
-        const int slot = id >> 3;
-        bh = (slot / ntile) * 8 + (id & 7);
-        tile = slot % ntile;
-        return bh < d.nbh;
-    }
-    bh = id / ntile;
-    tile = id % ntile;
-    return true;
+    const int lanes = d.xcd ? 8 : 1, id = d.xcd ? blockIdx.x >> 3 : blockIdx.x, heads = (d.nbh + lanes - 1) / lanes;
+    const int h = d.causal ? id % heads : id / ntile;
+    tile = d.causal ? id / heads : id % ntile;
+    bh = h * lanes + (d.xcd ? blockIdx.x & 7 : 0);
+    return bh < d.nbh;
 }
 static inline unsigned attn_grid(const AttnDims& d, int ntile) { return (unsigned)((d.xcd ? (d.nbh + 7) / 8 * 8 : d.nbh) * (long)ntile); }
 
