@@ -211,16 +211,11 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         sq.fetch(Q, rt * QT, rows, nch, tid);
         so.fetch(GO, rt * QT, rows, nch, tid);
         // the first QT threads: lse and limit; the next QT: delta
-        static_assert(2 * QT <= NT, "a thread per statistic");
-        if (tid < 2 * QT) {
-            const int r = rt * QT + tid % QT, t = (int)((unsigned)r / (unsigned)d.G);
-            st = 0.f;
-            sl = -1;
-            if (r < rows) {
-                const long at = ((long)b * d.H + hk * d.G + (r - t * d.G)) * d.Tq + t;
-                st = tid < QT ? a.lse[at] : a.delta[at];
-                sl = d.causal ? min(klen - 1, t + shift) : klen - 1;
-            }
+        static_assert(2 * QT <= NT && 2 * QT % 64 == 0, "a thread per statistic, whole waves");
+        if (__builtin_amdgcn_readfirstlane(wave) < 2 * QT / 64) {
+            const int r = rt * QT + tid % QT, rr = min(r, rows - 1), t = d.G == 1 ? rr : (int)((unsigned)rr / (unsigned)d.G);
+            st = (tid < QT ? a.lse : a.delta)[((long)b * d.H + hk * d.G + (rr - t * d.G)) * d.Tq + t];
+            sl = r >= rows ? -1 : d.causal ? min(klen - 1, t + shift) : klen - 1;
         }
     };
     if (rt0 < rt1) fetch(rt0);
@@ -277,7 +272,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             }
         }
         // a key of this workgroup is hidden from some row of the tile, or the tile is not full
-        const int t0 = (int)((unsigned)(rt * QT) / (unsigned)d.G), lim0 = d.causal ? min(klen - 1, t0 + shift) : klen - 1;
+        const int t0 = d.G == 1 ? rt * QT : (int)((unsigned)(rt * QT) / (unsigned)d.G), lim0 = d.causal ? min(klen - 1, t0 + shift) : klen - 1;
         if (__builtin_expect(key0 + OG * 32 - 1 > lim0 || (rt + 1) * QT > rows, 0)) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
