@@ -7,7 +7,7 @@
 //     lane, P goes from accumulator to operand in place;
 //   * a workgroup is four waves, OG row groups x SG key groups (4 x 1, 2 x 2, 1 x 4 for more than 64, more than 32 and up to 32 rows); the
 //     key tile staged in LDS is shared by the row groups and divided among the key groups, whose (O, m, l) meet in LDS at the end;
-//   * the next tile is in registers during the products;
+//   * the next tile is on its way during the products: straight into the other LDS buffer (16-bit types), else into registers;
 //   * rows behind a sequence's end and rows that see no key are zeros, with -inf; keys behind the end are not read;
 //   * few rows: the keys are split over workgroups in units of equal length whatever the sequences' lengths, each leaves (O, m, l) in f32,
 //     a second launch joins them.
@@ -112,8 +112,22 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
     const int lim = row < rows ? (d.causal ? min(klen - 1, tok + shift) : klen - 1) : -1;      // last visible key
     const int lim0 = d.causal ? min(klen - 1, tok0 + shift) : klen - 1;                         // ... of the workgroup's first row
 
-    Stager<T, DP, KT, NT> sk, sv;
-    if (kt0 < kt1) {
+    using ST = Stager<T, DP, KT, NT>;
+    constexpr bool DIRECT = ST::DIRECT && NB == 2;
+    const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    ST sk, sv;
+    auto direct = [&](int kt, int buf) {
+        char* t = smem + buf * 2 * TL::bytes(KT);
+        ST::direct(t, K, kt * KT, klen, nch, tid, uwave);
+        ST::direct(t + TL::bytes(KT), V, kt * KT, klen, nch, tid, uwave);
+    };
+    if constexpr (DIRECT) {
+        if (nch < TL::NCH) {
+            clear_lds<4 * TL::bytes(KT), NT>(smem, tid);
+            __syncthreads();
+        }
+        if (kt0 < kt1) direct(kt0, 0);
+    } else if (kt0 < kt1) {
         sk.fetch(K, kt0 * KT, klen, nch, tid);
         sv.fetch(V, kt0 * KT, klen, nch, tid);
     }
@@ -130,13 +144,19 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
 
     for (int kt = kt0, buf = 0; kt < kt1; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
-        if (NB == 1 && kt > kt0) __syncthreads();              // (with two buffers the other one's readers passed the barrier of the tile before)
-        sk.put(tk, tid);
-        sv.put(tv, tid);
-        __syncthreads();
-        if (kt + 1 < kt1) {
-            sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
-            sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
+        if constexpr (DIRECT) {
+            wait_direct();
+            __syncthreads();                                   // this tile is there, and the other buffer's readers are done
+            if (kt + 1 < kt1) direct(kt + 1, buf ^ 1);
+        } else {
+            if (NB == 1 && kt > kt0) __syncthreads();          // (with two buffers the other one's readers passed the barrier of the tile before)
+            sk.put(tk, tid);
+            sv.put(tv, tid);
+            __syncthreads();
+            if (kt + 1 < kt1) {
+                sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
+                sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
+            }
         }
         const int own = sg * MBW * 32;                         // this key group's rows of the tile
         f32x16 s[MBW];

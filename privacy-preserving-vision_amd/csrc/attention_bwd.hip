@@ -81,8 +81,22 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     const int lim = row < rows ? (d.causal ? min(klen - 1, tok + shift) : klen - 1) : -1;
     const int lim0 = d.causal ? min(klen - 1, tok0 + shift) : klen - 1;
 
-    Stager<T, DP, KT, NT> sk, sv;
-    if (ktiles) {
+    using ST = Stager<T, DP, KT, NT>;
+    constexpr bool DIRECT = ST::DIRECT && NB == 2;
+    const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    ST sk, sv;
+    auto direct = [&](int kt, int buf) {
+        char* t = smem + buf * 2 * TL::bytes(KT);
+        ST::direct(t, K, kt * KT, klen, nch, tid, uwave);
+        ST::direct(t + TL::bytes(KT), V, kt * KT, klen, nch, tid, uwave);
+    };
+    if constexpr (DIRECT) {
+        if (nch < TL::NCH) {
+            clear_lds<4 * TL::bytes(KT), NT>(smem, tid);
+            __syncthreads();
+        }
+        if (ktiles) direct(0, 0);
+    } else if (ktiles) {
         sk.fetch(K, 0, klen, nch, tid);
         sv.fetch(V, 0, klen, nch, tid);
     }
@@ -126,13 +140,19 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     const int own = sg * 32;                                   // this group's rows of a tile
     for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
-        if (NB == 1 && kt > 0) __syncthreads();
-        sk.put(tk, tid);
-        sv.put(tv, tid);
-        __syncthreads();
-        if (kt + 1 < ktiles) {
-            sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
-            sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
+        if constexpr (DIRECT) {
+            wait_direct();
+            __syncthreads();
+            if (kt + 1 < ktiles) direct(kt + 1, buf ^ 1);
+        } else {
+            if (NB == 1 && kt > 0) __syncthreads();
+            sk.put(tk, tid);
+            sv.put(tv, tid);
+            __syncthreads();
+            if (kt + 1 < ktiles) {
+                sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
+                sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
+            }
         }
         f32x16 s, p;
 #pragma unroll
@@ -204,21 +224,34 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     const int rt0 = key0 < klen ? (int)min((long)first * d.G, (long)rows) / QT : 0;
     const int rt1 = key0 < klen ? (rows + QT - 1) / QT : 0;
 
-    Stager<T, DP, QT, NT> sq, so;
+    using ST = Stager<T, DP, QT, NT>;
+    constexpr bool DIRECT = ST::DIRECT && NB == 2;
+    const int uwave = __builtin_amdgcn_readfirstlane(wave);
+    ST sq, so;
     float st = 0.f;
     int sl = -1;
-    auto fetch = [&](int rt) {
-        sq.fetch(Q, rt * QT, rows, nch, tid);
-        so.fetch(GO, rt * QT, rows, nch, tid);
+    if (DIRECT && nch < TL::NCH) {
+        clear_lds<DIRECT ? 4 * TL::bytes(QT) : NT * 16, NT>(smem, tid);
+        __syncthreads();
+    }
+    auto fetch = [&](int rt, int buf) {
+        if constexpr (DIRECT) {
+            char* t = smem + buf * 2 * TL::bytes(QT);
+            ST::direct(t, Q, rt * QT, rows, nch, tid, uwave);
+            ST::direct(t + TL::bytes(QT), GO, rt * QT, rows, nch, tid, uwave);
+        } else {
+            sq.fetch(Q, rt * QT, rows, nch, tid);
+            so.fetch(GO, rt * QT, rows, nch, tid);
+        }
         // the first QT threads: lse and limit; the next QT: delta
         static_assert(2 * QT <= NT && 2 * QT % 64 == 0, "a thread per statistic, whole waves");
-        if (__builtin_amdgcn_readfirstlane(wave) < 2 * QT / 64) {
+        if (uwave < 2 * QT / 64) {
             const int r = rt * QT + tid % QT, rr = min(r, rows - 1), t = d.G == 1 ? rr : (int)((unsigned)rr / (unsigned)d.G);
             st = (tid < QT ? a.lse : a.delta)[((long)b * d.H + hk * d.G + (rr - t * d.G)) * d.Tq + t];
             sl = r >= rows ? -1 : d.causal ? min(klen - 1, t + shift) : klen - 1;
         }
     };
-    if (rt0 < rt1) fetch(rt0);
+    if (rt0 < rt1) fetch(rt0, 0);
     u32x4 kf_[TL::NF], vf[VL ? 1 : TL::NF];
     load_own<T, DP>(kf_, K, key, klen, nch, lane);
     if constexpr (VL) {
@@ -238,14 +271,17 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     for (int rt = rt0, buf = 0; rt < rt1; ++rt, buf ^= NB - 1) {
         char *tq = smem + buf * 2 * TL::bytes(QT), *tg = tq + TL::bytes(QT);
         if (NB == 1 && rt > rt0) __syncthreads();
-        sq.put(tq, tid);
-        so.put(tg, tid);
+        if constexpr (DIRECT) wait_direct();
+        else {
+            sq.put(tq, tid);
+            so.put(tg, tid);
+        }
         if (tid < 2 * QT) {
             stat[buf][tid / QT][tid % QT] = st;
             if (tid < QT) limit[buf][tid] = sl;
         }
         __syncthreads();
-        if (rt + 1 < rt1) fetch(rt + 1);
+        if (rt + 1 < rt1) fetch(rt + 1, buf ^ 1);
         // (opaque in each turn: the 16 addresses made from it are then computed where they are used and not kept in 16 registers)
         auto L = L0;
         asm volatile("" : "+v"(L.row), "+v"(L.col0), "+v"(L.col1));
@@ -315,13 +351,13 @@ static int attn_groups(long n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
 
 template <class T, int DP> static int attn_bwd_t(AttnBwd a, hipStream_t stream) {
     const long rows = (long)a.d.Tq * a.d.G;
-    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;  // (one group that holds K, V, dK and dV of 128 f32 spills)
-    const int nq = attn_groups(rows), nk = attn_groups(a.d.Tk) < LEAST ? LEAST : attn_groups(a.d.Tk);
+    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;  // (one group that holds a row's or a key's part of 128 f32 spills)
+    const int nq = attn_groups(rows) < LEAST ? LEAST : attn_groups(rows), nk = attn_groups(a.d.Tk) < LEAST ? LEAST : attn_groups(a.d.Tk);
     a.ntile = (int)((rows + nq * 32 - 1) / (nq * 32));
     const int tk = (a.d.Tk + nk * 32 - 1) / (nk * 32);
     if ((long)a.d.nbh * a.ntile > 0x7ffffff0L || (long)a.d.nbh * tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
     unsigned grid = attn_grid(a.d, a.ntile);
-    if (nq == 1) attn_dq_kernel<T, DP, 1><<<grid, 256, 0, stream>>>(a);
+    if (nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
     else if (nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dq_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
     if (a.d.Tk == 0) return ppv_last_error();

@@ -184,7 +184,41 @@ template <class T, int DP, int ROWS, int NT> struct Stager {
             if (EVEN || idx < ALL) *reinterpret_cast<u32x4*>(tile + TL::at(idx / TL::NCH, idx % TL::NCH)) = v[i];
         }
     }
+
+    // The same without registers (16-bit types): whole tiles go from memory to LDS directly, complete after wait_direct() and a barrier.  A
+    // wave's 64 lanes fill 1024 consecutive bytes, so it is the SOURCE chunk that is permuted.  Chunks behind the head dimension are not
+    // written: the caller has cleared both tile buffers once.  A tile that is not whole goes through registers, zeros behind the end.
+    static constexpr bool DIRECT = sizeof(T) == 2 && EVEN && STEP % 16 == 0;
+    static __device__ __forceinline__ void direct(char* tile, const RowsOf<T>& src, int row0, int rows, int nch, int tid, int wave) {
+        const int r0 = tid / TL::NCH, ch = (tid % TL::NCH) ^ TL::key(r0);                  // (STEP is a multiple of 16: one key for all)
+        if (row0 + ROWS <= rows) {
+            if (ch < nch) {
+                const unsigned off = (unsigned)r0 * (unsigned)src.st * 2u + (unsigned)ch * 16u;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const char* p = src.G == 1 ? (const char*)(src.base + (long)(row0 + i * STEP) * src.st) + off
+                                               : (const char*)(src.row(row0 + i * STEP + r0) + ch * 8);
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                                     (__attribute__((address_space(3))) void*)(tile + (i * NT + wave * 64) * 16), 16, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = row0 + i * STEP + r0;
+                u32x4 x = {0, 0, 0, 0};
+                if (ch < nch && r < rows) x = *reinterpret_cast<const u32x4*>(src.row(r) + ch * 8);
+                *reinterpret_cast<u32x4*>(tile + (i * NT + tid) * 16) = x;
+            }
+        }
+    }
 };
+__device__ __forceinline__ void wait_direct() { __builtin_amdgcn_s_waitcnt(0x0F70); }      // vmcnt(0)
+template <int BYTES, int NT> __device__ __forceinline__ void clear_lds(char* p, int tid) {
+#pragma unroll
+    for (int i = 0; i < BYTES / (NT * 16); ++i) *reinterpret_cast<u32x4*>(p + (i * NT + tid) * 16) = (u32x4){0, 0, 0, 0};
+    static_assert(BYTES % (NT * 16) == 0, "whole sweeps");
+}
 // B operand fragments (n = row lane % 32 of 32 rows from row0, k along the head dimension), straight from memory
 template <class T, int DP> __device__ __forceinline__ void load_own(u32x4* f, const RowsOf<T>& src, int row, int rows, int nch, int lane) {
     const bool ok = row < rows;
