@@ -263,7 +263,7 @@ typedef struct {
 } PpvAttention;
 size_t ppv_attention_fwd_workspace_bytes(int B, int H, int Hkv, int Tq, int Tk, int D, int dtype);
 int ppv_attention_fwd(const PpvAttention* x, ppv_stream_t stream);
-size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Tq);
+size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Hkv, int Tq, int Tk, int D, int dtype);
 int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream);
 
 /* weight gradient (layer2..4 trainable, models.py:43-54): torch layout [N][Cs][R][S] f32 out; per-slice slabs in scratch */

@@ -201,7 +201,7 @@ class Attention(ctypes.Structure):
 
 PROTOTYPES["ppv_attention_fwd_workspace_bytes"] = (_Z, [_I] * 7)
 PROTOTYPES["ppv_attention_fwd"] = (_I, [ctypes.POINTER(Attention), _P])
-PROTOTYPES["ppv_attention_bwd_workspace_bytes"] = (_Z, [_I] * 3)
+PROTOTYPES["ppv_attention_bwd_workspace_bytes"] = (_Z, [_I] * 7)
 PROTOTYPES["ppv_attention_bwd"] = (_I, [ctypes.POINTER(Attention), _P])
 
 TRUNK_MAX_BLOCKS = 64

@@ -6,7 +6,8 @@
 // Two launches, no atomics: the gradients have the same bits every time.
 //   attn_dq   a wave owns 32 rows (columns of S^T, dP^T, dQ^T) and walks over the keys; it also leaves D for the second launch
 //   attn_dkv  a wave owns 32 keys (columns of S, dP, dK^T, dV^T) and walks over the rows of all query heads that share them
-// That is 7 products where one launch with atomics on dQ would need 5.  Bound by the matrix pipe and, behind it, the LDS: every operand of a
+// That is 7 products where one launch with atomics on dQ would need 5.  Where few rows (keys) leave the chip idle, the axis that is walked over is
+// split; the splits' f32 sums are added in their order by a small launch.  Bound by the matrix pipe and, behind it, the LDS: every operand of a
 // tile is read along its rows (S, dP) and across them (dQ, dK, dV).
 #include "attention_tiles.h"
 
@@ -19,8 +20,17 @@ struct AttnBwd {
     const float* lse;                                          // [B][H][Tq], log2
     float* delta;                                              // [B][H][Tq]
     void *dq, *dk, *dv;
-    int ntile;
+    float* part;                                               // nsplit > 1: f32 sums [nsplit][nbh][rows or Tk][DP] (dK, then dV)
+    int ntile, nsplit;
 };
+
+// a split's share [t0, t1) of the tiles that a workgroup walks over
+__device__ __forceinline__ void attn_share(int nsplit, int& t0, int& t1) {
+    if (nsplit == 1) return;
+    const int per = (t1 - t0 + nsplit - 1) / nsplit;
+    t0 = min(t1, t0 + per * (int)blockIdx.y);
+    t1 = min(t1, t0 + per);
+}
 
 // four waves: OG groups that own 32 columns each x SG groups that divide a staged tile's rows, whose sums meet in LDS at the end
 template <class T, int DP, int OG, int ACC> struct BwdShape {
@@ -77,7 +87,8 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     int kend = klen;
     if (d.causal) kend = min(klen, max(0, (int)((unsigned)max(last, 0) / (unsigned)d.G) + shift + 1));
     if (row0 >= rows) kend = 0;
-    const int ktiles = (kend + KT - 1) / KT;
+    int kt0 = 0, kt1 = (kend + KT - 1) / KT;
+    attn_share(a.nsplit, kt0, kt1);
     const int lim = row < rows ? (d.causal ? min(klen - 1, tok + shift) : klen - 1) : -1;
     const int lim0 = d.causal ? min(klen - 1, tok0 + shift) : klen - 1;
 
@@ -95,10 +106,10 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
             clear_lds<4 * TL::bytes(KT), NT>(smem, tid);
             __syncthreads();
         }
-        if (ktiles) direct(0, 0);
-    } else if (ktiles) {
-        sk.fetch(K, 0, klen, nch, tid);
-        sv.fetch(V, 0, klen, nch, tid);
+        if (kt0 < kt1) direct(kt0, 0);
+    } else if (kt0 < kt1) {
+        sk.fetch(K, kt0 * KT, klen, nch, tid);
+        sv.fetch(V, kt0 * KT, klen, nch, tid);
     }
     u32x4 qf[TL::NF], gf[TL::NF];
     load_own<T, DP>(qf, Q, row, rows, nch, lane);
@@ -127,7 +138,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     float lse = 0.f;
     if (row < rows) {
         lse = a.lse[stat];
-        if (half == 0 && sg == 0) a.delta[stat] = delta;
+        if (half == 0 && sg == 0 && blockIdx.y == 0) a.delta[stat] = delta;
     }
     const float c = d.scale * LOG2E;
     f32x16 acc[TL::DB];
@@ -138,18 +149,18 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
 
     const auto L = TL::lane_part(lane);
     const int own = sg * 32;                                   // this group's rows of a tile
-    for (int kt = 0, buf = 0; kt < ktiles; ++kt, buf ^= NB - 1) {
+    for (int kt = kt0, buf = 0; kt < kt1; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
         if constexpr (DIRECT) {
             wait_direct();
             __syncthreads();
-            if (kt + 1 < ktiles) direct(kt + 1, buf ^ 1);
+            if (kt + 1 < kt1) direct(kt + 1, buf ^ 1);
         } else {
-            if (NB == 1 && kt > 0) __syncthreads();
+            if (NB == 1 && kt > kt0) __syncthreads();
             sk.put(tk, tid);
             sv.put(tv, tid);
             __syncthreads();
-            if (kt + 1 < ktiles) {
+            if (kt + 1 < kt1) {
                 sk.fetch(K, (kt + 1) * KT, klen, nch, tid);
                 sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
             }
@@ -183,6 +194,15 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     for (int i = 0; i < TL::DB; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = lim < 0 ? 0.f : acc[i][j] * d.scale;      // (rows that see nothing: zeros, whatever K holds)
+    if (a.nsplit > 1) {
+        float* po = a.part + (((long)blockIdx.y * d.nbh + bh) * d.Tq * d.G + row) * DP;
+#pragma unroll
+        for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store4<float>(po + i * 32 + g * 8 + half * 4, acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]);
+        return;
+    }
     T* po = (T*)a.dq + (((long)b * d.Tq + tok) * d.H + h) * d.D;
 #pragma unroll
     for (int i = 0; i < TL::DB; ++i)
@@ -221,8 +241,9 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
 
     // rows that see a key of this workgroup
     const int first = d.causal ? max(0, key0 - shift) : 0;     // (token)
-    const int rt0 = key0 < klen ? (int)min((long)first * d.G, (long)rows) / QT : 0;
-    const int rt1 = key0 < klen ? (rows + QT - 1) / QT : 0;
+    int rt0 = key0 < klen ? (int)min((long)first * d.G, (long)rows) / QT : 0;
+    int rt1 = key0 < klen ? (rows + QT - 1) / QT : 0;
+    attn_share(a.nsplit, rt0, rt1);
 
     using ST = Stager<T, DP, QT, NT>;
     constexpr bool DIRECT = ST::DIRECT && NB == 2;
@@ -334,6 +355,19 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     if (SG > 1) __syncthreads();
     if (!meet<TL::DB, OG, SG>(dv, (float*)smem, og, sg, lane) || !first_group) return;
     if (key >= d.Tk) return;
+    if (a.nsplit > 1) {
+        float* pk = a.part + (((long)blockIdx.y * d.nbh + bh) * d.Tk + key) * DP;
+        float* pv = pk + (long)a.nsplit * d.nbh * d.Tk * DP;
+#pragma unroll
+        for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int e = i * 32 + g * 8 + half * 4;
+                store4<float>(pk + e, dk[i][4 * g] * d.scale, dk[i][4 * g + 1] * d.scale, dk[i][4 * g + 2] * d.scale, dk[i][4 * g + 3] * d.scale);
+                store4<float>(pv + e, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+            }
+        return;
+    }
     const long at = (((long)b * d.Tk + key) * d.Hkv + hk) * d.D;
 #pragma unroll
     for (int i = 0; i < TL::DB; ++i)
@@ -347,29 +381,77 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         }
 }
 
-static int attn_groups(long n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; }
+// the splits' sums, added in their order: part [nsplit][nbh][n][DP] -> out; n rows of G heads (dQ) or n keys (G = 1, `heads` = Hkv)
+template <class T, int DP> __global__ __launch_bounds__(256) void attn_split_sum_kernel(const float* __restrict__ part, T* __restrict__ out, int nsplit, int nbh,
+                                                                                       int Hkv, int G, int n, int D) {
+    constexpr int PER = DP / 4;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, at = i / PER;
+    const int e = (int)(i % PER) * 4;
+    if (at >= (long)nbh * n || e >= D) return;
+    float4 s = *reinterpret_cast<const float4*>(part + at * DP + e);
+    for (int k = 1; k < nsplit; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(part + ((long)k * nbh * n + at) * DP + e);
+        s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    const int bh = (int)(at / n), r = (int)(at % n), b = bh / Hkv, tok = r / G, h = (bh - b * Hkv) * G + (r - tok * G);
+    store4<T>(out + (((long)b * (n / G) + tok) * Hkv * G + h) * D + e, s.x, s.y, s.z, s.w);
+}
 
-template <class T, int DP> static int attn_bwd_t(AttnBwd a, hipStream_t stream) {
-    const long rows = (long)a.d.Tq * a.d.G;
-    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;  // (one group that holds a row's or a key's part of 128 f32 spills)
-    const int nq = attn_groups(rows) < LEAST ? LEAST : attn_groups(rows), nk = attn_groups(a.d.Tk) < LEAST ? LEAST : attn_groups(a.d.Tk);
-    a.ntile = (int)((rows + nq * 32 - 1) / (nq * 32));
-    const int tk = (a.d.Tk + nk * 32 - 1) / (nk * 32);
-    if ((long)a.d.nbh * a.ntile > 0x7ffffff0L || (long)a.d.nbh * tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
-    unsigned grid = attn_grid(a.d, a.ntile);
-    if (nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
-    else if (nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
+// groups that own rows (keys), tiles of them, ways to split the other axis
+struct BwdPlan { int nq, nk, tq, tk, sq, sk, dp; size_t part; };
+static BwdPlan attn_bwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int es) {
+    BwdPlan p;
+    p.dp = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+    const int least = es == 4 && p.dp == 128 ? 2 : 1;          // (one group that holds a row's or a key's part of 128 f32 spills)
+    auto groups = [&](long n) { return n <= 32 && least == 1 ? 1 : n <= 64 ? 2 : 4; };
+    const long rows = (long)Tq * G, bh = (long)B * Hkv;
+    p.nq = groups(rows);
+    p.nk = groups(Tk);
+    p.tq = (int)((rows + p.nq * 32 - 1) / (p.nq * 32));
+    p.tk = (Tk + p.nk * 32 - 1) / (p.nk * 32);
+    // where the tiles alone leave the chip idle, the other axis is split: at most 512 workgroups, at least four of its tiles each
+    auto ways = [&](long base, long walk, int own) {
+        long s = base >= 256 ? 1 : 512 / base;
+        const long most = walk / (32 * (4 / own)) / 4;
+        s = s > most ? most : s;
+        return (int)(s < 2 ? 1 : s);
+    };
+    p.sq = ways(bh * p.tq, Tk, p.nq);
+    p.sk = p.tk ? ways(bh * p.tk, rows, p.nk) : 1;
+    const size_t q = p.sq > 1 ? (size_t)p.sq * bh * rows * p.dp : 0, k = p.sk > 1 ? (size_t)p.sk * bh * Tk * p.dp * 2 : 0;
+    p.part = (q > k ? q : k) * sizeof(float);                  // (dQ's sums are used up before dK's are made)
+    return p;
+}
+
+template <class T, int DP> static int attn_bwd_t(AttnBwd a, const BwdPlan& p, hipStream_t stream) {
+    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;
+    const AttnDims& d = a.d;
+    if ((long)d.nbh * p.tq > 0x7ffffff0L || (long)d.nbh * p.tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
+    auto sum = [&](const float* part, void* out, int nsplit, int G, int n) {
+        attn_split_sum_kernel<T, DP><<<(unsigned)(((long)d.nbh * n * (DP / 4) + 255) / 256), 256, 0, stream>>>(part, (T*)out, nsplit, d.nbh, d.Hkv, G, n, d.D);
+    };
+    a.ntile = p.tq;
+    a.nsplit = p.sq;
+    dim3 grid(attn_grid(d, p.tq), p.sq);
+    if (p.nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
+    else if (p.nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dq_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
-    if (a.d.Tk == 0) return ppv_last_error();
-    a.ntile = tk;
-    grid = attn_grid(a.d, tk);
-    if (nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
-    else if (nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
+    if (p.sq > 1) sum(a.part, a.dq, p.sq, d.G, d.Tq * d.G);
+    if (d.Tk == 0) return ppv_last_error();
+    a.ntile = p.tk;
+    a.nsplit = p.sk;
+    grid = dim3(attn_grid(d, p.tk), p.sk);
+    if (p.nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
+    else if (p.nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dkv_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
+    if (p.sk > 1) {
+        sum(a.part, a.dk, p.sk, 1, d.Tk);
+        sum(a.part + (size_t)p.sk * d.nbh * d.Tk * DP, a.dv, p.sk, 1, d.Tk);
+    }
     return ppv_last_error();
 }
-template <class T> static int attn_bwd_dp(const AttnBwd& a, hipStream_t stream) {
-    return a.d.D <= 32 ? attn_bwd_t<T, 32>(a, stream) : a.d.D <= 64 ? attn_bwd_t<T, 64>(a, stream) : attn_bwd_t<T, 128>(a, stream);
+template <class T> static int attn_bwd_dp(const AttnBwd& a, const BwdPlan& p, hipStream_t stream) {
+    return p.dp == 32 ? attn_bwd_t<T, 32>(a, p, stream) : p.dp == 64 ? attn_bwd_t<T, 64>(a, p, stream) : attn_bwd_t<T, 128>(a, p, stream);
 }
 
 }  // namespace ppv
@@ -378,8 +460,12 @@ using namespace ppv;
 
 extern "C" {
 
-size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Tq) {
-    return B < 1 || H < 1 || Tq < 1 ? 0 : (size_t)B * H * Tq * sizeof(float);
+// delta [B][H][Tq] f32 (rounded up to 16 bytes), then the splits' sums
+static size_t delta_bytes(int B, int H, int Tq) { return ((size_t)B * H * Tq * sizeof(float) + 15) / 16 * 16; }
+
+size_t ppv_attention_bwd_workspace_bytes(int B, int H, int Hkv, int Tq, int Tk, int D, int dtype) {
+    if (B < 1 || Hkv < 1 || H < Hkv || H % Hkv || Tq < 1 || Tk < 0 || D < 1 || D > 128 || dtype < 0 || dtype > 2) return 0;
+    return delta_bytes(B, H, Tq) + attn_bwd_plan(B, Hkv, H / Hkv, Tq, Tk, D, dtype == 0 ? 4 : 2).part;
 }
 
 int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
@@ -393,7 +479,7 @@ int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
     for (long s : st)
         if (s < 0 || s % v) return PPV_ERR_BAD_SIZE;
     if (x->sgt > 1 << 22) return PPV_ERR_BAD_SIZE;
-    const void* ps[] = {x->dout, x->dq, x->dk, x->dv};
+    const void* ps[] = {x->dout, x->dq, x->dk, x->dv, x->workspace};
     for (const void* p : ps)
         if ((size_t)p % 16) return PPV_ERR_BAD_SIZE;
     a.q = {x->q, x->sqb, x->sqt, x->sqh};
@@ -404,10 +490,12 @@ int ppv_attention_bwd(const PpvAttention* x, ppv_stream_t stream) {
     a.out_lo = x->out_lo;
     a.lse = x->lse;
     a.delta = (float*)x->workspace;
+    a.part = (float*)((char*)x->workspace + delta_bytes(x->B, x->H, x->Tq));
+    const BwdPlan p = attn_bwd_plan(x->B, x->Hkv, a.d.G, x->Tq, x->Tk, x->D, x->dtype == 0 ? 4 : 2);
     a.dq = x->dq;
     a.dk = x->dk;
     a.dv = x->dv;
-    return x->dtype == 0 ? attn_bwd_dp<float>(a, stream) : x->dtype == 1 ? attn_bwd_dp<bf16s>(a, stream) : attn_bwd_dp<f16s>(a, stream);
+    return x->dtype == 0 ? attn_bwd_dp<float>(a, p, stream) : x->dtype == 1 ? attn_bwd_dp<bf16s>(a, p, stream) : attn_bwd_dp<f16s>(a, p, stream);
 }
 
 }  // extern "C"

@@ -238,7 +238,7 @@ struct Attention : torch::autograd::Function<Attention> {
                 a.dout = g.data_ptr();
                 a.sgb = stride_of(g, 0); a.sgt = stride_of(g, 1); a.sgh = stride_of(g, 2);
                 a.dq = d[0].data_ptr(); a.dk = d[1].data_ptr(); a.dv = d[2].data_ptr();
-                const Tensor ws = at::empty({(int64_t)abi.attention_bwd_ws(a.B, a.H, a.Tq)}, q.options().dtype(at::kByte));
+                const Tensor ws = at::empty({(int64_t)abi.attention_bwd_ws(a.B, a.H, a.Hkv, a.Tq, a.Tk, a.D, a.dtype)}, q.options().dtype(at::kByte));
                 a.workspace = ws.data_ptr();
                 check(abi.attention_bwd(&a, stream()), "ppv_attention_bwd");
             }

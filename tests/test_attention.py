@@ -152,6 +152,19 @@ def test_attention_few_rows_against_many_keys(B, Tq, Tk, H, Hkv, D, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hkv,D", [(1, 900, 40, 4, 1, 64), (1, 40, 1500, 1, 1, 128), (1, 1100, 1100, 1, 1, 48), (2, 500, 130, 8, 2, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_gradients_where_the_walk_is_split(B, Tq, Tk, H, Hkv, D, causal, dt):
+    """Few tiles own rows or keys: the other axis is split over workgroups, ragged, so that some splits have nothing to do."""
+    q, k, v, g = _inputs(B, Tq, Tk, H, Hkv, D, DT[dt], Tq + D)
+    q_lens = torch.tensor([Tq - 333 * b - 7 for b in range(B)], dtype=torch.int32)
+    k_lens = torch.tensor([Tk - 90 * b for b in range(B)], dtype=torch.int32)
+    want, tol = _bounds(q, k, v, g, causal, q_lens, k_lens, None)
+    _check(NAMES, _run(q, k, v, g, causal=causal, q_lens=q_lens, k_lens=k_lens), want, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_attention_large_scores(dt):
     """Scores of several hundred: the softmax is a choice of one key; equal scores share; a lone enormous score wins without an overflow."""
@@ -313,7 +326,7 @@ def test_attention_entry_points_refuse():
         assert L.ppv_attention_fwd(args(**kw), None) == SIZE, kw
     for kw in ({"sgt": 12}, {"dout": 72}, {"dk": 8}):
         assert L.ppv_attention_bwd(args(**kw), None) == SIZE, kw
-    assert L.ppv_attention_fwd_workspace_bytes(1, 3, 2, 1, 1, 8, 1) == 0 and L.ppv_attention_bwd_workspace_bytes(0, 1, 1) == 0
+    assert L.ppv_attention_fwd_workspace_bytes(1, 3, 2, 1, 1, 8, 1) == 0 and L.ppv_attention_bwd_workspace_bytes(0, 1, 1, 1, 1, 8, 1) == 0
 
 
 @pytest.mark.gpu
