@@ -53,37 +53,32 @@ template <class T> __device__ __forceinline__ u32x4 pack_vec(const float (&v)[16
     return r;
 }
 
-// the 16 bytes at p as they are (any alignment of T); elements at or behind `left` are zeros and are not touched
-template <class T> __device__ __forceinline__ u32x4 load_raw(const T* p, int left) {
+// Vectors of a row of C elements without conditions: column c of the row is asked for at min(c, C - V), so the row's last vector, which may not
+// be whole, lies inside the row and every lane loads; `drop` = c - min(c, C - V) elements are then taken off its front, with zeros behind
+// (V or more: all zeros).  Loads under a condition are waited for one by one.  C < V: element by element.
+template <class T> __device__ __forceinline__ u32x4 load_row_vec(const T* row, int c, int C) {
     constexpr int V = 16 / sizeof(T);
-    if (left >= V) return *reinterpret_cast<const typename Raw16<T>::type*>(p);
+    if (C >= V) return *reinterpret_cast<const typename Raw16<T>::type*>(row + min(c, C - V));
     u32x4 r = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < V; ++e)
-        if (e < left) {
-            if constexpr (sizeof(T) == 4) r[e] = *reinterpret_cast<const unsigned*>(p + e);
-            else r[e / 2] |= (unsigned)p[e].u << (16 * (e & 1));
+        if (c + e < C) {
+            if constexpr (sizeof(T) == 4) r[e] = *reinterpret_cast<const unsigned*>(row + c + e);
+            else r[e / 2] |= (unsigned)row[c + e].u << (16 * (e & 1));
         }
     return r;
 }
-// the 16 / sizeof(T) elements at p (any alignment of T); those at or behind `left` read as zero and are not touched
-template <class T, int V> __device__ __forceinline__ void load_vec(const T* p, int left, float (&o)[V]) {
-    if (left >= V) {
-        if constexpr (V * sizeof(T) == 16) unpack_vec<T>(*reinterpret_cast<const typename Raw16<T>::type*>(p), o);
-        else if constexpr (V * sizeof(T) == 32) {
-            float lo[V / 2], hi[V / 2];
-            unpack_vec<T>(*reinterpret_cast<const typename Raw16<T>::type*>(p), lo);
-            unpack_vec<T>(*reinterpret_cast<const typename Raw16<T>::type*>(p + V / 2), hi);
-#pragma unroll
-            for (int e = 0; e < V / 2; ++e) { o[e] = lo[e]; o[V / 2 + e] = hi[e]; }
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = to_f32(p[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = e < left ? to_f32(p[e]) : 0.f;
-    }
+template <class T> __device__ __forceinline__ u32x4 drop_front(u32x4 r, int drop) {
+    constexpr int V = 16 / sizeof(T);
+    if (sizeof(T) == 2 && (drop & 1)) r = (u32x4){r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+    if (drop & (V / 4)) r = (u32x4){r[1], r[2], r[3], 0};
+    if (drop & (V / 2)) r = (u32x4){r[2], r[3], 0, 0};
+    return drop >= V ? (u32x4){0, 0, 0, 0} : r;
+}
+template <class T, int V> __device__ __forceinline__ void load_row(const T* row, int c, int C, float (&o)[V]) {
+    u32x4 r = load_row_vec<T>(row, c, C);
+    if (C >= V && __builtin_amdgcn_ballot_w64(c > C - V)) r = drop_front<T>(r, c - min(c, C - V));
+    unpack_vec<T>(r, o);
 }
 template <class T, int V> __device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[V]) {
     static_assert(V * sizeof(T) == 16, "one 16-byte vector");
@@ -94,14 +89,41 @@ template <class T, int V> __device__ __forceinline__ void store_vec(T* p, int le
             if (e < left) p[e] = from_f32<T>(v[e]);
     }
 }
-// a parameter vector of run-time type (0 f32, 1 bf16, 2 f16); `fill` where there is none and behind the end
-template <int V> __device__ __forceinline__ void load_param(const void* p, int dtype, long at, int left, float fill, float (&o)[V]) {
-    if (p == nullptr || left <= 0) {
+// V elements at column c of a parameter row of run-time type (0 f32, 1 bf16, 2 f16), as load_row_vec; `fill` where there is none, anything behind C
+template <class T, int V> __device__ __forceinline__ void load_param_t(const T* p, int c, int C, float (&o)[V]) {
+    constexpr int W = 16 / sizeof(T);                          // V is W, 2 W (f32 beside 16-bit rows) or W / 2 (16-bit beside f32 rows)
+    if (C >= V) {
+        const int at = min(c, C - V), drop = c - at;
+        if constexpr (V >= W) {
+#pragma unroll
+            for (int k = 0; k < V / W; ++k) {
+                float x[W];
+                unpack_vec<T>(*reinterpret_cast<const typename Raw16<T>::type*>(p + at + k * W), x);
+#pragma unroll
+                for (int e = 0; e < W; ++e) o[k * W + e] = x[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = to_f32(p[at + e]);
+        }
+        if (__builtin_amdgcn_ballot_w64(drop > 0 && drop < V)) {
+#pragma unroll
+            for (int bit = 1; bit < V; bit *= 2)
+#pragma unroll
+                for (int e = 0; e < V; ++e) o[e] = (drop & bit) && e + bit < V ? o[e + bit] : o[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = c + e < C ? to_f32(p[c + e]) : 0.f;
+    }
+}
+template <int V> __device__ __forceinline__ void load_param(const void* p, int dtype, int c, int C, float fill, float (&o)[V]) {
+    if (p == nullptr) {
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = fill;
-    } else if (dtype == 0) load_vec<float, V>((const float*)p + at, left, o);
-    else if (dtype == 1) load_vec<bf16s, V>((const bf16s*)p + at, left, o);
-    else load_vec<f16s, V>((const f16s*)p + at, left, o);
+    } else if (dtype == 0) load_param_t<float, V>((const float*)p, c, C, o);
+    else if (dtype == 1) load_param_t<bf16s, V>((const bf16s*)p, c, C, o);
+    else load_param_t<f16s, V>((const f16s*)p, c, C, o);
 }
 __device__ __forceinline__ void store_param(void* p, int dtype, long at, float v) {
     if (dtype == 0) ((float*)p)[at] = v;

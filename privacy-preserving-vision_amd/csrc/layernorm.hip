@@ -46,12 +46,16 @@ __global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__
     const long row = (long)blockIdx.x * RPW + threadIdx.x / LPR;
     const bool live = row < rows;                              // (a dead group keeps running: the sums below cross lanes)
     const T* xr = x + (live ? row : 0) * ldx;
+    u32x4 raw[NV];
     float v[NV][V];
     float s = 0.f;
 #pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = load_row_vec<T>(xr, (i * LPR + l) * V, C);
+#pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * LPR + l) * V;
-        load_vec<T, V>(xr + c, C - c, v[i]);
+        if ((i + 1) * LPR * V > C && C >= V) raw[i] = drop_front<T>(raw[i], c - min(c, C - V));
+        unpack_vec<T>(raw[i], v[i]);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -63,9 +67,11 @@ __global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int left = C - (i * LPR + l) * V;
+        const bool end = (i + 1) * LPR * V > C;                // (the same for all lanes: the other vectors are whole)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            v[i][e] = e < left ? v[i][e] - mean : 0.f;
+            v[i][e] -= mean;
+            if (end && e >= left) v[i][e] = 0.f;
             q = __builtin_fmaf(v[i][e], v[i][e], q);
         }
     }
@@ -77,8 +83,8 @@ __global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__
         const int c = (i * LPR + l) * V;
         if (c >= C) continue;
         float wv[V], bv[V], o[V];
-        load_param<V>(w, wdtype, c, C - c, 1.f, wv);
-        load_param<V>(b, wdtype, c, C - c, 0.f, bv);
+        load_param<V>(w, wdtype, c, C, 1.f, wv);
+        load_param<V>(b, wdtype, c, C, 0.f, bv);
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(v[i][e] * rstd, wv[e], bv[e]);
         store_vec<T, V>(yr + c, C - c, o);
@@ -98,13 +104,13 @@ __global__ __launch_bounds__(256) void layernorm_fwd_long_kernel(const T* __rest
     float v[V];
     float s = 0.f, q = 0.f;
     for (int c = threadIdx.x * V; c < C; c += 256 * V) {
-        load_vec<T, V>(xr + c, C - c, v);
+        load_row<T, V>(xr, c, C, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) s += v[e];
     }
     const float mean = group_sum<256>(s, lds) / (float)C;
     for (int c = threadIdx.x * V; c < C; c += 256 * V) {
-        load_vec<T, V>(xr + c, C - c, v);
+        load_row<T, V>(xr, c, C, v);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const float d = e < C - c ? v[e] - mean : 0.f;
@@ -115,9 +121,9 @@ __global__ __launch_bounds__(256) void layernorm_fwd_long_kernel(const T* __rest
     T* yr = y + row * (long)C;
     for (int c = threadIdx.x * V; c < C; c += 256 * V) {
         float wv[V], bv[V];
-        load_vec<T, V>(xr + c, C - c, v);
-        load_param<V>(w, wdtype, c, C - c, 1.f, wv);
-        load_param<V>(b, wdtype, c, C - c, 0.f, bv);
+        load_row<T, V>(xr, c, C, v);
+        load_param<V>(w, wdtype, c, C, 1.f, wv);
+        load_param<V>(b, wdtype, c, C, 0.f, bv);
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = __builtin_fmaf((v[e] - mean) * rstd, wv[e], bv[e]);
         store_vec<T, V>(yr + c, C - c, v);
@@ -162,8 +168,8 @@ __global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restric
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * LPR + l) * V;
-            gr[i] = load_raw<T>(g + at * ldg + c, live ? C - c : 0);
-            xr[i] = load_raw<T>(x + at * ldx + c, live ? C - c : 0);
+            gr[i] = load_row_vec<T>(g + at * ldg, c, C);
+            xr[i] = load_row_vec<T>(x + at * ldx, c, C);
         }
         mean = mean_in[at];
         rstd = rstd_in[at];
@@ -173,7 +179,7 @@ __global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restric
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * LPR + l) * V;
-        load_param<V>(w, wdtype, c, C - c, 1.f, wv[i]);
+        load_param<V>(w, wdtype, c, C, 1.f, wv[i]);
 #pragma unroll
         for (int e = 0; e < V; ++e) aw[i][e] = ab[i][e] = 0.f;
     }
@@ -183,6 +189,12 @@ __global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restric
         float gv[NV][V], hv[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            if ((i + 1) * LPR * V > C && C >= V) {
+                gr[i] = drop_front<T>(gr[i], c - min(c, C - V));
+                xr[i] = drop_front<T>(xr[i], c - min(c, C - V));
+            }
+            if (!live) gr[i] = (u32x4){0, 0, 0, 0};            // (this slot's last turn may have no row)
             unpack_vec<T>(gr[i], gv[i]);
             unpack_vec<T>(xr[i], hv[i]);
         }
@@ -192,10 +204,12 @@ __global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restric
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int left = live ? C - (i * LPR + l) * V : 0;
+            const int left = C - (i * LPR + l) * V;
+            const bool end = (i + 1) * LPR * V > C;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float h = e < left ? (hv[i][e] - mu) * rs : 0.f, gw = gv[i][e] * wv[i][e];       // (g is zero behind the row)
+                float h = (hv[i][e] - mu) * rs, gw = gv[i][e] * wv[i][e];                              // (g is zero behind the row)
+                if (end && e >= left) h = gw = 0.f;
                 aw[i][e] = __builtin_fmaf(gv[i][e], h, aw[i][e]);
                 ab[i][e] += gv[i][e];
                 s1 += gw;
@@ -273,9 +287,9 @@ __global__ __launch_bounds__(256) void layernorm_bwd_long_kernel(const T* __rest
     for (int pass = 0; pass < 2; ++pass) {
         for (int c = threadIdx.x * V; c < C; c += 256 * V) {
             float gv[V], xv[V], wv[V];
-            load_vec<T, V>(g + row * ldg + c, C - c, gv);
-            load_vec<T, V>(x + row * ldx + c, C - c, xv);
-            load_param<V>(w, wdtype, c, C - c, 1.f, wv);
+            load_row<T, V>(g + row * ldg, c, C, gv);
+            load_row<T, V>(x + row * ldx, c, C, xv);
+            load_param<V>(w, wdtype, c, C, 1.f, wv);
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
