@@ -6,12 +6,13 @@
 // Byte-bound: forward reads x and writes y, backward reads x and g and writes dx, once each.  A row is held in registers by LPR lanes
 // (16, a wave, or a workgroup), NV 16-byte vectors each, so the variance is the two-pass one (sum of squared distances from the mean: no
 // cancellation for rows far from zero) without reading the row again.  All sums are f32.  Rows may start at any element: the 16-byte
-// loads ask for element alignment only (global memory takes them), the last vector of a row is taken element by element.
-// Backward: a fixed grid strides over the rows, the next row's operands are on their way while one is worked on, every lane keeps the
-// weight-gradient sums of its columns in registers, a workgroup leaves one partial row, a second launch adds the partial rows in their order (no atomics:
+// loads ask for element alignment only (global memory takes them), the last vector of a row is read from where it is whole (elem_types.h).
+// Both directions: a fixed grid strides over the rows, the parameters are in registers, the next row is on its way while one is worked on.
+// Backward: every lane keeps the weight-gradient sums of its columns in registers, a workgroup leaves one partial row, a second launch adds the partial rows in their order (no atomics:
 // the same bits every time).
-// Measured (MI355X): 165888 rows of 2048 bf16, forward 245 us = 5.5 TB/s, backward 370 us = 5.5 TB/s (without the next row's loads, 32
-// elements a lane: 560); 6656 rows of 512: 5 + 11 + 4 us, less than the host takes to ask for them.
+// Measured (MI355X, bytes read and written once): 165888 x 2048 bf16 forward 5.4 TB/s, backward 5.5 (620 us together; 560 for backward alone without
+// the next row's loads); f32 5.0-5.7 and 4.9-5.6 at any C; 16-bit rows of an odd C, which start off every dword, 4 and 2.6-4.4; rows longer than
+// 8192, read again for each pass, 2.4-3.4 and 1.6-2.5.  6656 x 512 bf16: 5 + 8 + 4 us, less than the host takes to ask for them.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include "ppv_common.h"
@@ -28,9 +29,10 @@ template <int LPR> __device__ __forceinline__ float group_sum(float v, float* ld
         constexpr int NW = LPR / 64;
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = lds[0];
+        const int w0 = threadIdx.x / LPR * NW;
+        v = lds[w0];
 #pragma unroll
-        for (int i = 1; i < NW; ++i) v += lds[i];
+        for (int i = 1; i < NW; ++i) v += lds[w0 + i];
         __syncthreads();                                       // the next sum writes the same words
     }
     return v;
@@ -41,55 +43,66 @@ __global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__
                                                            int wdtype, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                                            long rows, int C, float eps) {
     constexpr int V = 16 / sizeof(T), RPW = NT / LPR;
-    __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
-    const int l = threadIdx.x % LPR;
-    const long row = (long)blockIdx.x * RPW + threadIdx.x / LPR;
-    const bool live = row < rows;                              // (a dead group keeps running: the sums below cross lanes)
-    const T* xr = x + (live ? row : 0) * ldx;
-    u32x4 raw[NV];
-    float v[NV][V];
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = load_row_vec<T>(xr, (i * LPR + l) * V, C);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + l) * V;
-        if ((i + 1) * LPR * V > C && C >= V) raw[i] = drop_front<T>(raw[i], c - min(c, C - V));
-        unpack_vec<T>(raw[i], v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < V; ++e) s += v[i][e];
+    __shared__ float lds[LPR > 64 ? NT / 64 : 1];
+    const int l = threadIdx.x % LPR, grp = threadIdx.x / LPR;
     const float inv_c = 1.f / (float)C;
-    const float mean = group_sum<LPR>(s, lds) * inv_c;
-    float q = 0.f;
+    const long step = (long)gridDim.x * RPW, turns = (rows + step - 1) / step, row0 = (long)blockIdx.x * RPW + grp;
+    u32x4 raw[NV];
+    auto fetch = [&](long row) {
+        const T* xr = x + (row < rows ? row : 0) * ldx;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) raw[i] = load_row_vec<T>(xr, (i * LPR + l) * V, C);
+    };
+    fetch(row0);
+    float wv[NV][V], bv[NV][V];                                // once for all rows of this slot
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int left = C - (i * LPR + l) * V;
-        const bool end = (i + 1) * LPR * V > C;                // (the same for all lanes: the other vectors are whole)
+        load_param<V>(w, wdtype, (i * LPR + l) * V, C, 1.f, wv[i]);
+        load_param<V>(b, wdtype, (i * LPR + l) * V, C, 0.f, bv[i]);
+    }
+    for (long t = 0; t < turns; ++t) {                         // (a slot without a row keeps running: the sums below cross lanes)
+        const long row = t * step + row0;
+        float v[NV][V];
+        float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            v[i][e] -= mean;
-            if (end && e >= left) v[i][e] = 0.f;
-            q = __builtin_fmaf(v[i][e], v[i][e], q);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            if ((i + 1) * LPR * V > C && C >= V) raw[i] = drop_front<T>(raw[i], c - min(c, C - V));
+            unpack_vec<T>(raw[i], v[i]);
         }
-    }
-    const float rstd = 1.f / __builtin_sqrtf(group_sum<LPR>(q, lds) * inv_c + eps);
-    if (!live) return;
-    T* yr = y + row * (long)C;
+        if (t + 1 < turns) fetch(row + step);                  // the next row comes while this one is worked on
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + l) * V;
-        if (c >= C) continue;
-        float wv[V], bv[V], o[V];
-        load_param<V>(w, wdtype, c, C, 1.f, wv);
-        load_param<V>(b, wdtype, c, C, 0.f, bv);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(v[i][e] * rstd, wv[e], bv[e]);
-        store_vec<T, V>(yr + c, C - c, o);
+            for (int e = 0; e < V; ++e) s += v[i][e];
+        const float mean = group_sum<LPR>(s, lds) * inv_c;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int left = C - (i * LPR + l) * V;
+            const bool end = (i + 1) * LPR * V > C;            // (the same for all lanes: the other vectors are whole)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[i][e] -= mean;
+                if (end && e >= left) v[i][e] = 0.f;
+                q = __builtin_fmaf(v[i][e], v[i][e], q);
+            }
+        }
+        const float rstd = 1.f / __builtin_sqrtf(group_sum<LPR>(q, lds) * inv_c + eps);
+        if (row >= rows) continue;
+        T* yr = y + row * (long)C;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * LPR + l) * V;
+            if (c >= C) continue;
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(v[i][e] * rstd, wv[i][e], bv[i][e]);
+            store_vec<T, V>(yr + c, C - c, o);
+        }
+        if (mean_out && l == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
     }
-    if (mean_out && l == 0) { mean_out[row] = mean; rstd_out[row] = rstd; }
 }
 
 // rows longer than the registers hold: three passes over the row (the second and third come out of the L2)
@@ -331,7 +344,7 @@ __global__ __launch_bounds__(256) void layernorm_wgrad_reduce_kernel(const float
     const long c = (long)blockIdx.x * 16 + j;                  // over the 2 C columns of a partial row
     float a = 0.f;
     if (c < 2L * C) {
-#pragma unroll 4
+#pragma unroll 8
         for (int r = k; r < G; r += 16) a += part[(long)r * 2 * C + c];
     }
     s[k][j] = a;
@@ -351,33 +364,35 @@ static int layernorm_bwd_groups(long rows, int C, int rpw) {
     const long most = C > 8192 ? 64 : 512;
     return (int)(by_rows < 1 ? 1 : by_rows > most ? most : by_rows);
 }
-// lanes per row of the backward kernels: at most 16 elements a lane (two gradient sums, a weight and two operands each; with 32 the next row's
+// lanes per row: at most 16 elements a lane (two gradient sums, a weight and two operands each; with 32 the next row's
 // loads no longer fit beside them), 0: longer than the registers hold
-static int layernorm_bwd_lpr(int C, int dtype) {
+static int layernorm_lpr(int C, int dtype) {
     const int v = dtype == 0 ? 4 : 8, nvec = (C + v - 1) / v, most = 16 / v;
     return nvec <= 16 ? 16 : nvec <= 64 * most ? 64 : nvec <= 128 * most ? 128 : nvec <= 256 * most ? 256 : nvec <= 512 * most ? 512 : 0;
 }
 static int layernorm_groups_of(long rows, int C, int dtype) {
-    const int lpr = layernorm_bwd_lpr(C, dtype);
+    const int lpr = layernorm_lpr(C, dtype);
     return layernorm_bwd_groups(rows, C, lpr == 0 || lpr >= 256 ? 1 : 256 / lpr);
 }
 
+constexpr long FWD_GROUPS = 1024;
 template <class T>
 static int layernorm_fwd_t(const T* x, long ldx, const void* w, const void* b, int wdtype, T* y, float* mean, float* rstd, long rows, int C,
                            float eps, hipStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    const int nvec = (C + V - 1) / V;
-    auto grid = [&](int rpw) { return (rows + rpw - 1) / rpw; };
-    if (grid(16) > 0x7fffffffL || (nvec > 16 && grid(4) > 0x7fffffffL) || (nvec > 512 && rows > 0x7fffffffL)) return PPV_ERR_BAD_SIZE;
+    const int nvec = (C + V - 1) / V, lpr = layernorm_lpr(C, sizeof(T) == 4 ? 0 : 1);
+    // four workgroups of 256 threads for each CU, each with as many rows as that takes (2048 and more are no faster)
+    auto grid = [&](int rpw, long most) { const long n = (rows + rpw - 1) / rpw; return (unsigned)(n < most ? n : most); };
 #define LN_FWD(LPR, NV, NT) \
-    layernorm_fwd_kernel<T, LPR, NV, NT><<<(unsigned)grid(NT / LPR), NT, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, rows, C, eps)
-    if (nvec <= 16) LN_FWD(16, 1, 256);
-    else if (nvec <= 64) LN_FWD(64, 1, 256);
-    else if (nvec <= 128) LN_FWD(64, 2, 256);
-    else if (nvec <= 256) LN_FWD(64, 4, 256);
-    else if (nvec <= 512) LN_FWD(64, 8, 256);
-    else if (nvec <= 1024) LN_FWD(256, 4, 256);
-    else if (nvec <= 2048) LN_FWD(256, 8, 256);
+    layernorm_fwd_kernel<T, LPR, NV, NT><<<grid(NT / LPR, NT == 512 ? 1024 : FWD_GROUPS), NT, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, rows, C, eps)
+    if (lpr == 16) LN_FWD(16, 1, 256);
+    else if (lpr == 64 && nvec <= 64) LN_FWD(64, 1, 256);
+    else if (lpr == 64 && nvec <= 128) LN_FWD(64, 2, 256);
+    else if (lpr == 64) LN_FWD(64, 16 / V, 256);               // (f32: 4 vectors; the 16-bit types end at 2)
+    else if (lpr == 128) LN_FWD(128, 16 / V, 256);
+    else if (lpr == 256) LN_FWD(256, 16 / V, 256);
+    else if (lpr == 512) LN_FWD(512, 16 / V, 512);
+    else if (rows > 0x7fffffffL) return PPV_ERR_BAD_SIZE;
     else layernorm_fwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, C, eps);
 #undef LN_FWD
     return ppv_last_error();
@@ -387,7 +402,7 @@ template <class T>
 static int layernorm_bwd_t(const T* g, long ldg, const T* x, long ldx, const void* w, int wdtype, const float* mean, const float* rstd, T* dx,
                            void* dw, void* db, float* part, long rows, int C, int dtype, hipStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    const int nvec = (C + V - 1) / V, lpr = layernorm_bwd_lpr(C, dtype), G = layernorm_groups_of(rows, C, dtype);
+    const int nvec = (C + V - 1) / V, lpr = layernorm_lpr(C, dtype), G = layernorm_groups_of(rows, C, dtype);
     if (!dw && !db) part = nullptr;
 #define LN_BWD(LPR, NV, NT)                                                                                                              \
     layernorm_bwd_kernel<T, LPR, NV, NT><<<G, NT, (LPR >= NT ? 0 : LPR <= 64 ? NT / 64 : NT / LPR) * C * sizeof(float), stream>>>(        \
