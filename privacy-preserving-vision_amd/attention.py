@@ -51,6 +51,8 @@ def multihead_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=N
         raise ValueError(f"multihead_attention: shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
     if H < 1 or k.shape[2] < 1 or H % k.shape[2]:
         raise ValueError(f"multihead_attention: {H} query heads over {k.shape[2]} key heads")
+    if max(B * k.shape[2], Tq * H, k.shape[1]) >= 1 << 30:
+        raise ValueError("multihead_attention: fewer than 2^30 rows, keys and (sequence, key head) pairs")
     if not 1 <= D <= 128:
         raise ValueError(f"multihead_attention: head dimension {D} is not in 1..128")
     scale = D ** -0.5 if scale is None else float(scale)

@@ -1,7 +1,9 @@
 // Multi-head attention, backward (gfx950).  P is computed again from Q, K and the saved log-sum-exp; nothing of size Tq x Tk is stored:
 //
-//     P = exp2(scale log2e Q K^T - lse),   dP = dO V^T,   D = rowsum(dO O),   dS = P (dP - D)
-//     dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
+//     P = exp2(scale log2e Q K^T - lse),   dP = dO V^T,   D = scale rowsum(dO O),   dS = P (scale dP - D)
+//     dQ = dS K,   dK = dS^T Q,   dV = P^T dO
+//
+// (The scale is in dS when it is rounded to the operands' type: its range in f16 is then that of the results.)
 //
 // Two launches, no atomics: the gradients have the same bits every time.
 //   attn_dq   a wave owns 32 rows (columns of S^T, dP^T, dQ^T) and walks over the keys; it also leaves D for the second launch
@@ -18,7 +20,7 @@ struct AttnBwd {
     AttnTensor q, k, v, g;                                     // g: dO
     const void *out, *out_lo;
     const float* lse;                                          // [B][H][Tq], log2
-    float* delta;                                              // [B][H][Tq]
+    float* delta;                                              // [B][H][Tq]: scale rowsum(dO O)
     void *dq, *dk, *dv;
     float* part;                                               // nsplit > 1: f32 sums [nsplit][nbh][rows or Tk][DP] (dK, then dV)
     int ntile, nsplit;
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     };
     delta = dot(a.out);
     if (a.out_lo) delta += dot(a.out_lo);                      // O as the forward pass had it: its rounding would be dS's largest error
-    delta = half_swap_sum(delta);
+    delta = half_swap_sum(delta) * d.scale;
     const int h = hk * d.G + (row - tok * d.G);
     const long stat = ((long)b * d.H + h) * d.Tq + tok;
     float lse = 0.f;
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
             p = TL::mma(TL::by_row(tv, L, own, kd), gf[kd], p);
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * (p[j] - delta);
+        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * __builtin_fmaf(p[j], d.scale, -delta);
         if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
 #pragma unroll
     for (int i = 0; i < TL::DB; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[i][j] = lim < 0 ? 0.f : acc[i][j] * d.scale;      // (rows that see nothing: zeros, whatever K holds)
+        for (int j = 0; j < 16; ++j) acc[i][j] = lim < 0 ? 0.f : acc[i][j];      // (rows that see nothing: zeros, whatever K holds)
     if (a.nsplit > 1) {
         float* po = a.part + (((long)blockIdx.y * d.nbh + bh) * d.Tq * d.G + row) * DP;
 #pragma unroll
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             for (int i = 0; i < 4; ++i) {
                 const int j = 4 * g + i;
                 const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lsv[i]));
-                s[j] = pe * (p[j] - dev[i]);
+                s[j] = pe * __builtin_fmaf(p[j], d.scale, -dev[i]);
                 p[j] = pe;
             }
         }
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int e = i * 32 + g * 8 + half * 4;
-                store4<float>(pk + e, dk[i][4 * g] * d.scale, dk[i][4 * g + 1] * d.scale, dk[i][4 * g + 2] * d.scale, dk[i][4 * g + 3] * d.scale);
+                store4<float>(pk + e, dk[i][4 * g], dk[i][4 * g + 1], dk[i][4 * g + 2], dk[i][4 * g + 3]);
                 store4<float>(pv + e, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
             }
         return;
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         for (int g = 0; g < 4; ++g) {
             const int e = i * 32 + g * 8 + half * 4;
             if (e < d.D) {
-                store4<T>((T*)a.dk + at + e, dk[i][4 * g] * d.scale, dk[i][4 * g + 1] * d.scale, dk[i][4 * g + 2] * d.scale, dk[i][4 * g + 3] * d.scale);
+                store4<T>((T*)a.dk + at + e, dk[i][4 * g], dk[i][4 * g + 1], dk[i][4 * g + 2], dk[i][4 * g + 3]);
                 store4<T>((T*)a.dv + at + e, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
             }
         }

@@ -236,8 +236,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps): x [..., C] f32, bf16 or f16 with any strides and any C >= 1,
     weight / bias [C] (or None) of one of those types, both of the same one; the result has x's type, statistics and sums are f32.
     Gradients to x, weight and bias (once differentiable, deterministic: the weight gradient's partial sums are added in a fixed order)."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("layer_norm: x is [..., C] with C >= 1")
+    if x.dim() < 1 or not 1 <= x.shape[-1] < 1 << 30:
+        raise ValueError("layer_norm: x is [..., C] with 1 <= C < 2^30")
     if x.dtype not in ELEM_TYPES:
         raise TypeError(f"layer_norm: x is f32, bf16 or f16, not {x.dtype}")
     for name, t in (("weight", weight), ("bias", bias)):

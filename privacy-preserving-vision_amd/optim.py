@@ -216,7 +216,7 @@ class AdamW(torch.optim.Optimizer):
                 del self._tables[k]
             b1, b2 = group["betas"]
             for slot, (t, sub) in enumerate(sorted(by_step.items())):
-                self._list((gi, slot), sub).step(group["lr"], b1, b2, group["eps"], group["weight_decay"], t + 1.0, self.seed & 0xFFFFFFFF)
+                self._list((gi, slot), sub).step(float(group["lr"]), b1, b2, group["eps"], group["weight_decay"], t + 1.0, self.seed & 0xFFFFFFFF)
                 for p in sub:
                     self.state[p]["step"] = t + 1.0
         return loss

@@ -6,7 +6,7 @@ Tolerances count roundings.  u = 2^-24 (f32 arithmetic), h = half a step of the 
      maximum, exp2 and the saved log-sum-exp add (4 + |S| + log) u.  So P is off by eP = e_s + h relative, e_s = u (D + 2) max(scale |q||k|) + 32 u.
   O = sum P V: |dO_i| <= (eP + (Tk + 8) u ... a f32 chain over tiles, counted as 64 u + Tk / 32 u) sum P |V|, then rounded once: h |O|.
   dV = sum P dO likewise.  dS = P (dP - D) with dP, D off by (D + 2) u |dO||V| and, D being taken from the rounded O, h |dO| . |O|;
-     rounded to the operands' type: h.  dQ and dK sum dS over keys and rows."""
+     rounded to the operands' type with the scale in it: h.  dQ and dK sum dS over keys and rows."""
 import math
 
 import pytest
@@ -61,7 +61,7 @@ def _bounds(q, k, v, g, causal, q_lens, k_lens, scale):
         delta = (gb * ob).sum(-1, keepdim=True)
         e_dp = (D + 2) * U * gb.norm(dim=-1, keepdim=True) * vb.norm(dim=-1).amax()
         e_delta = (gb.abs() * (hr * ob.abs() + (eP + eS) * o_sum)).sum(-1, keepdim=True) + (D + 2) * U * (gb.abs() * ob.abs()).sum(-1, keepdim=True)
-        e_ds = p * ((dp - delta).abs() * (es + h + 4 * U) + e_dp + e_delta) + tiny
+        e_ds = p * ((dp - delta).abs() * (es + h + 4 * U) + e_dp + e_delta) + tiny / scale           # (rounded with the scale in it)
         ds = (p * (dp - delta)).abs()
         rows = n * G
         eR = 64 * U + rows / 32 * U
@@ -220,6 +220,19 @@ def test_attention_strides_and_layouts():
             ones = torch.ones((), dtype=dt)
             want, tol = _bounds(q, k, v, ones.expand(g.shape), False, None, None, None)
             _check(NAMES, (out.detach(),) + torch.autograd.grad(out.sum(), leaves), want, tol)
+
+
+@pytest.mark.gpu
+def test_attention_gradients_of_a_scaled_loss_in_f16():
+    """dO of several thousand (a loss multiplied for f16): dO V^T leaves f16's range, the gradients do not."""
+    q, k, v, g = _inputs(1, 70, 90, 2, 2, 128, torch.float16, 12)
+    g = g * 3000.0
+    v = v * 2.0
+    want, tol = _bounds(q, k, v, g, False, None, None, None)
+    got = _run(q, k, v, g)
+    assert (g.double().view(70, 2, 128).transpose(0, 1) @ v.double().view(90, 2, 128).permute(1, 2, 0)).abs().max() > 65504
+    assert all(torch.isfinite(t).all() for t in got)
+    _check(NAMES, got, want, tol)
 
 
 @pytest.mark.gpu
