@@ -162,14 +162,17 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
             }
         }
         const int own = sg * MBW * 32;                         // this key group's rows of the tile
+        __builtin_amdgcn_s_setprio(1);
         f32x16 s[MBW];
 #pragma unroll
-        for (int mb = 0; mb < MBW; ++mb) {
+        for (int mb = 0; mb < MBW; ++mb)
 #pragma unroll
             for (int j = 0; j < 16; ++j) s[mb][j] = 0.f;
 #pragma unroll
-            for (int kd = 0; kd < TL::NF; ++kd) s[mb] = TL::mma(TL::by_row(tk, L, own + mb * 32, kd), qf[kd], s[mb]);
-        }
+        for (int kd = 0; kd < TL::NF; ++kd)
+#pragma unroll
+            for (int mb = 0; mb < MBW; ++mb) s[mb] = TL::mma(TL::by_row(tk, L, own + mb * 32, kd), qf[kd], s[mb]);
+        __builtin_amdgcn_s_setprio(0);
         if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
 #pragma unroll
             for (int mb = 0; mb < MBW; ++mb)
@@ -204,6 +207,7 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
                 sum += s[mb][j];
             }
         l += sum;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int mb = 0; mb < MBW; ++mb)
 #pragma unroll
@@ -212,6 +216,7 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
 #pragma unroll
                 for (int i = 0; i < TL::DB; ++i) o[i] = TL::mma(TL::by_col(tv, L, own + mb * 32, i, kf), pf, o[i]);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     l = half_swap_sum(l);
     if constexpr (SG > 1) {                                    // the key groups' shares of the same rows, added in their order

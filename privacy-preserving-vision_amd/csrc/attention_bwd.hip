@@ -37,8 +37,8 @@ __device__ __forceinline__ void attn_share(int nsplit, int& t0, int& t1) {
 }
 
 // four waves: OG groups that own 32 columns each x SG groups that divide a staged tile's rows, whose sums meet in LDS at the end
-template <class T, int DP, int OG, int ACC> struct BwdShape {
-    static constexpr int SG = 4 / OG, KT = 32 * SG;
+template <class T, int DP, int OG, int ACC, int MB = 1> struct BwdShape {
+    static constexpr int SG = 4 / OG, KT = 32 * SG * MB;        // (MB blocks of 32 rows for each group, one after the other)
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
@@ -68,7 +68,8 @@ template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* a
 template <class T, int DP, int OG>
 __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_kernel(const AttnBwd a) {
     using TL = Tile<T, DP>;
-    using SH = BwdShape<T, DP, OG, 1>;
+    constexpr int MB = OG == 4 && sizeof(T) == 2 ? 2 : 1;
+    using SH = BwdShape<T, DP, OG, 1, MB>;
     constexpr int NT = 256, KT = SH::KT, NB = SH::NB, SG = SH::SG;
     __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
     const AttnDims& d = a.d;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
 
     const auto L = TL::lane_part(lane);
-    const int own = sg * 32;                                   // this group's rows of a tile
+    const int own = sg * MB * 32;                              // this group's rows of a tile
     for (int kt = kt0, buf = 0; kt < kt1; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
         if constexpr (DIRECT) {
@@ -169,28 +170,36 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
                 sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
             }
         }
-        f32x16 s, p;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
+        for (int mb = 0; mb < MB; ++mb) {
+            const int at = own + mb * 32;
+            __builtin_amdgcn_s_setprio(1);
+            f32x16 s, p;
 #pragma unroll
-        for (int kd = 0; kd < TL::NF; ++kd) {
-            s = TL::mma(TL::by_row(tk, L, own, kd), qf[kd], s);
-            p = TL::mma(TL::by_row(tv, L, own, kd), gf[kd], p);
-        }
+            for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * __builtin_fmaf(p[j], d.scale, -delta);
-        if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
+            for (int kd = 0; kd < TL::NF; ++kd) {
+                s = TL::mma(TL::by_row(tk, L, at, kd), qf[kd], s);
+                p = TL::mma(TL::by_row(tv, L, at, kd), gf[kd], p);
+            }
+            __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (kt * KT + own + 8 * (j >> 2) + 4 * half + (j & 3) > lim) s[j] = 0.f;
-        }
+            for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * __builtin_fmaf(p[j], d.scale, -delta);
+            if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
 #pragma unroll
-        for (int kf = 0; kf < TL::CF; ++kf) {
-            const u32x4 df = TL::from_acc(s, kf);
+                for (int j = 0; j < 16; ++j)
+                    if (kt * KT + at + 8 * (j >> 2) + 4 * half + (j & 3) > lim) s[j] = 0.f;
+            }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, L, own, i, kf), df, acc[i]);
+            for (int kf = 0; kf < TL::CF; ++kf) {
+                const u32x4 df = TL::from_acc(s, kf);
+#pragma unroll
+                for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, L, at, i, kf), df, acc[i]);
+            }
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (SG > 1) __syncthreads();
     if (!meet<TL::DB, OG, SG>(acc, (float*)smem, og, sg, lane)) return;
     if (row >= d.Tq * d.G) return;
@@ -310,6 +319,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         // (opaque in each turn: the 16 addresses made from it are then computed where they are used and not kept in 16 registers)
         auto L = L0;
         asm volatile("" : "+v"(L.row), "+v"(L.col0), "+v"(L.col1));
+        __builtin_amdgcn_s_setprio(1);
         f32x16 s, p;
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
@@ -319,6 +329,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             if constexpr (VL) p = TL::mma(TL::by_row(tg, L, own, kd), TL::by_row(vown, L, og * 32, kd), p);
             else p = TL::mma(TL::by_row(tg, L, own, kd), vf[kd], p);
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int r = own + 8 * g + 4 * half;
@@ -344,6 +355,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
                     if (key > liv[i]) p[4 * g + i] = s[4 * g + i] = 0.f;
             }
         }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int kf = 0; kf < TL::CF; ++kf) {
             const u32x4 pf = TL::from_acc(p, kf), df = TL::from_acc(s, kf);
@@ -354,6 +366,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             }
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (SG > 1) __syncthreads();
     const bool first_group = meet<TL::DB, OG, SG>(dk, (float*)smem, og, sg, lane);
     if (SG > 1) __syncthreads();
