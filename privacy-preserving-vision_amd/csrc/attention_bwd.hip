@@ -37,8 +37,8 @@ __device__ __forceinline__ void attn_share(int nsplit, int& t0, int& t1) {
 }
 
 // four waves: OG groups that own 32 columns each x SG groups that divide a staged tile's rows, whose sums meet in LDS at the end
-template <class T, int DP, int OG, int ACC, int MB = 1> struct BwdShape {
-    static constexpr int SG = 4 / OG, KT = 32 * SG * MB;        // (MB blocks of 32 rows for each group, one after the other)
+template <class T, int DP, int OG, int ACC> struct BwdShape {
+    static constexpr int SG = 4 / OG, KT = 32 * SG;
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
@@ -68,8 +68,7 @@ template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* a
 template <class T, int DP, int OG>
 __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_kernel(const AttnBwd a) {
     using TL = Tile<T, DP>;
-    constexpr int MB = OG == 4 && sizeof(T) == 2 ? 2 : 1;
-    using SH = BwdShape<T, DP, OG, 1, MB>;
+    using SH = BwdShape<T, DP, OG, 1>;
     constexpr int NT = 256, KT = SH::KT, NB = SH::NB, SG = SH::SG;
     __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
     const AttnDims& d = a.d;
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
 
     const auto L = TL::lane_part(lane);
-    const int own = sg * MB * 32;                              // this group's rows of a tile
+    const int own = sg * 32;                                   // this group's rows of a tile
     for (int kt = kt0, buf = 0; kt < kt1; ++kt, buf ^= NB - 1) {
         char *tk = smem + buf * 2 * TL::bytes(KT), *tv = tk + TL::bytes(KT);
         if constexpr (DIRECT) {
@@ -170,33 +169,29 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
                 sv.fetch(V, (kt + 1) * KT, klen, nch, tid);
             }
         }
+        __builtin_amdgcn_s_setprio(1);
+        f32x16 s, p;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-            const int at = own + mb * 32;
-            __builtin_amdgcn_s_setprio(1);
-            f32x16 s, p;
+        for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] = p[j] = 0.f;
+        for (int kd = 0; kd < TL::NF; ++kd) {
+            s = TL::mma(TL::by_row(tk, L, own, kd), qf[kd], s);
+            p = TL::mma(TL::by_row(tv, L, own, kd), gf[kd], p);
+        }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-            for (int kd = 0; kd < TL::NF; ++kd) {
-                s = TL::mma(TL::by_row(tk, L, at, kd), qf[kd], s);
-                p = TL::mma(TL::by_row(tv, L, at, kd), gf[kd], p);
-            }
-            __builtin_amdgcn_s_setprio(0);
+        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * __builtin_fmaf(p[j], d.scale, -delta);
+        if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
 #pragma unroll
-            for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lse)) * __builtin_fmaf(p[j], d.scale, -delta);
-            if (__builtin_expect(kt * KT + KT - 1 > lim0, 0)) {    // a key of this tile is hidden from some row
+            for (int j = 0; j < 16; ++j)
+                if (kt * KT + own + 8 * (j >> 2) + 4 * half + (j & 3) > lim) s[j] = 0.f;
+        }
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (kt * KT + at + 8 * (j >> 2) + 4 * half + (j & 3) > lim) s[j] = 0.f;
-            }
-            __builtin_amdgcn_s_setprio(1);
+        for (int kf = 0; kf < TL::CF; ++kf) {
+            const u32x4 df = TL::from_acc(s, kf);
 #pragma unroll
-            for (int kf = 0; kf < TL::CF; ++kf) {
-                const u32x4 df = TL::from_acc(s, kf);
-#pragma unroll
-                for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, L, at, i, kf), df, acc[i]);
-            }
+            for (int i = 0; i < TL::DB; ++i) acc[i] = TL::mma(TL::by_col(tk, L, own, i, kf), df, acc[i]);
         }
     }
     __builtin_amdgcn_s_setprio(0);
