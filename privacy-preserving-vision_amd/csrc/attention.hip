@@ -66,7 +66,7 @@ template <int KT> __device__ __forceinline__ void attn_units(const AttnDims& d, 
 
 template <class T, int DP, int OG> struct FwdShape {
     static constexpr int SG = 4 / OG, MBW = OG == 4 && sizeof(T) == 2 ? 2 : 1, KT = 32 * SG * MBW;
-    static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;                 // tile buffers
+    static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 81920 ? 2 : 1;                 // tile buffers
     static constexpr int PARK = (SG - 1) * OG * (DP / 2 + 2) * 256;                        // where the key groups meet
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
     static constexpr int WAVES = DP == 128 && sizeof(T) == 4 ? 1 : 2;         // per SIMD: 512 or 256 registers

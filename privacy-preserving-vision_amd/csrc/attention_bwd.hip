@@ -39,7 +39,7 @@ __device__ __forceinline__ void attn_share(int nsplit, int& t0, int& t1) {
 // four waves: OG groups that own 32 columns each x SG groups that divide a staged tile's rows, whose sums meet in LDS at the end
 template <class T, int DP, int OG, int ACC> struct BwdShape {
     static constexpr int SG = 4 / OG, KT = 32 * SG;
-    static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 65536 ? 2 : 1;
+    static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 81920 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
     static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG < ACC * 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
