@@ -7,11 +7,16 @@
 // there is one copy of it.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/utils/pybind.h>
+
+#include <unordered_set>
 
 #include "ppv_hip.h"
 
@@ -63,6 +68,33 @@ variable_list once(variable_list grads) {
     return error(std::move(in));
 }
 
+// A backward pass that is captured into a graph must not go on to a node of the default stream: the engine would make that stream wait for the
+// captured one, which no capture allows, and the broken capture ends the process when its graph is destroyed.  Such a node is the accumulation of a
+// leaf whose eager graph still lives, possibly some views away.
+void refuse_capture_of_eager_graph() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto* wanted = torch::autograd::get_current_graph_task_exec_info();              // (empty: all of the graph)
+    auto runs = [&](torch::autograd::Node* n) {
+        if (!wanted || wanted->empty()) return true;
+        const auto at = wanted->find(n);
+        return at != wanted->end() && at->second.should_execute();
+    };
+    const auto node = torch::autograd::get_current_node();
+    std::vector<torch::autograd::Node*> todo{node.get()};
+    std::unordered_set<torch::autograd::Node*> seen{node.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node* n = todo.back();
+        todo.pop_back();
+        for (const auto& e : n->next_edges())
+            if (e.function && runs(e.function.get()) && seen.insert(e.function.get()).second) {
+                const auto s = e.function->stream();
+                TORCH_CHECK(!s || s->id() != 0, "ppv_amd: this backward pass is being captured into a graph, but ", e.function->name(),
+                            " belongs to an eager graph of the default stream; drop that graph (or make it on a side stream) first");
+                todo.push_back(e.function.get());
+            }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------------- layer norm
 
 Tensor rows_of(const Tensor& t, int64_t C) {
@@ -100,6 +132,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         variable_list r;
         {
             at::NoGradGuard off;
+            refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
             const Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2], &g = grads[0];
             c10::DeviceGuard guard(x2.device());
@@ -224,6 +257,7 @@ struct Attention : torch::autograd::Function<Attention> {
         variable_list r(7);
         {
             at::NoGradGuard off;
+            refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
             const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3];
             c10::DeviceGuard guard(q.device());

@@ -229,3 +229,36 @@ def test_layer_norm_is_differentiable_once():
     assert torch.equal(dx, want)
     with pytest.raises(RuntimeError, match="differentiable once"):
         dx.sum().backward()
+
+
+@pytest.mark.gpu
+def test_captured_backward_over_a_living_eager_graph_is_refused():
+    """The engine would hand the gradient to the default stream, where the leaf's accumulation lives, in the middle of the capture: an error that says so
+    comes first, the capture stays whole and so does the eager graph.  Once the eager graph is gone, or where its leaf is not asked for, capturing works."""
+    from ppv_amd.attention import multihead_attention
+    from ppv_amd.nn_ops import layer_norm
+    torch.manual_seed(5)
+    x = torch.randn(6, 64, device="cuda", requires_grad=True)
+    w = torch.randn(64, device="cuda", requires_grad=True)
+    g = torch.randn(6, 64, device="cuda")
+    want = torch.autograd.grad(layer_norm(x, w), (x, w), g)
+    eager = layer_norm(x.view(6, 64), w) * 1.0
+    for run, what in ((lambda: torch.autograd.grad(layer_norm(x.view(6, 64), None), x, g), "layer norm"),
+                      (lambda: torch.autograd.grad(multihead_attention(*(x.view(1, 6, 1, 64),) * 3), x, g.view(1, 6, 1, 64)), "attention")):
+        graph, refused = torch.cuda.CUDAGraph(), ""
+        with torch.cuda.graph(graph):
+            scratch = torch.empty(4, device="cuda").zero_()     # (a capture that holds something)
+            try:
+                run()
+            except RuntimeError as e:
+                refused = str(e)
+        assert "eager graph" in refused and scratch.numel() == 4, what
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, (x, w), g), want))
+    eager = layer_norm(g, w)                                    # of w alone: x's graph is gone, w's is not asked for
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, = torch.autograd.grad(layer_norm(x, w), x, g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want[0]) and eager.requires_grad
