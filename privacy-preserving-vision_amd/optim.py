@@ -152,6 +152,10 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
+        ps = self.param_groups[-1]["params"]
+        if len(set(ps)) != len(ps):             # (two records of one tensor in the one launch would race)
+            del self.param_groups[-1]
+            raise ValueError("ppv_amd.optim.AdamW: a parameter appears twice in a group")
         self._number()
 
     def _number(self):
@@ -188,6 +192,9 @@ class AdamW(torch.optim.Optimizer):
             if not (all(t.device == p.device and t.is_contiguous() and t.numel() == n and t.dtype == kind for t in (m, v)) and (ms is None or all(
                     t.device == p.device and t.is_contiguous() and t.numel() == (n + 255) // 256 and t.dtype == torch.float32 for t in (ms, vs)))):
                 raise ValueError("ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)")
+        at = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in ps if p.numel())
+        if any(a[1] > b[0] for a, b in zip(at, at[1:])):
+            raise ValueError("ppv_amd.optim.AdamW: parameters of one group share memory")
         native = _lib.torch_ops().AdamWList(ps, held[0::4], held[1::4], held[2::4], held[3::4], [self._place[p] & 0xFFFFFFFF for p in ps])
         self._tables[slot] = (ps, held, native)
         return native
@@ -199,6 +206,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for gi, group in enumerate(self.param_groups):
+            if group["amsgrad"] or group["maximize"]:           # (a group's own, or a loaded one's)
+                raise NotImplementedError("ppv_amd.optim.AdamW: amsgrad / maximize are not implemented")
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
                 continue

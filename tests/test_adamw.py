@@ -298,3 +298,44 @@ def test_adamw_refuses_on_the_gpu():
         except RuntimeError:
             refused = True
     assert refused and o.state[q]["step"] == 1.0 and scratch.numel() == 4
+
+
+def test_adamw_refuses_a_group_that_asks_for_more():
+    """amsgrad and maximize of a single group, or of a state that was another optimiser's: refused, not left out."""
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    for name in ("amsgrad", "maximize"):
+        with pytest.raises(NotImplementedError, match="maximize"):
+            AdamW([{"params": [p], name: True}]).step()
+        o = AdamW([p])
+        o.load_state_dict(torch.optim.AdamW([p], **{name: True}).state_dict())
+        with pytest.raises(NotImplementedError, match="maximize"):
+            o.step()
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_adamw_refuses_a_parameter_twice():
+    from ppv_amd.optim import AdamW
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="twice"):
+        AdamW([p, q, p])
+    o = AdamW([p])
+    with pytest.raises(ValueError):
+        o.add_param_group({"params": [q, q]})
+    assert len(o.param_groups) == 1
+    with pytest.raises(ValueError):
+        o.add_param_group({"params": [q, p]})                   # (torch's own check)
+
+
+@pytest.mark.gpu
+def test_adamw_refuses_parameters_that_share_memory():
+    from ppv_amd.optim import AdamW
+    x = torch.zeros(100, device="cuda")
+    a, b, c = torch.nn.Parameter(x[:60]), torch.nn.Parameter(x[59:90]), torch.nn.Parameter(x[60:])
+    for t in (a, b, c):
+        t.grad = torch.ones_like(t)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([c, a, b]).step()
+    AdamW([c, a], lr=0.5, weight_decay=0.0).step()              # neighbours
+    assert (x + 0.5).abs().max() < 1e-6
