@@ -243,7 +243,7 @@ int ppv_layernorm_bwd(const void* g, long ldg, const void* x, long ldx, const vo
  * out = softmax(scale q k^T over the visible keys) v.  q, dout [B][Tq][H][D] and k, v [B][Tk][Hkv][D] by their strides in elements (batch, token,
  * head; the last axis has stride 1); out, dq [B][Tq][H][D] and dk, dv [B][Tk][Hkv][D] packed.  H is a multiple of Hkv: query head h reads
  * key head h / (H / Hkv).  dtype 0 f32, 1 bf16, 2 f16 of all of them; D <= 128 and every stride a multiple of 16 bytes, every address too; token strides at
- * most 2^22 elements.
+ * most 2^22 elements.  Fewer than 2^24 tiles of 32 to 128 rows (or keys) of one (sequence, key head), and than 2^30 tiles of 32 keys of all sequences.
  * q_lens, k_lens: DEVICE int32 [B] or NULL (Tq, Tk); values are clamped to 0..Tq, 0..Tk.  Row i < q_len sees key j < k_len, where causal if
  * j <= i + k_len - q_len.  Rows at or behind q_len and rows that see nothing give zeros (and zero gradients); keys at or behind k_len are
  * not read and get zero gradients.  lse [B][H][Tq] f32: log2 of the softmax's denominator, written by the forward pass (or NULL) and read by the

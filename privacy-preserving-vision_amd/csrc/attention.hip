@@ -376,7 +376,7 @@ static AttnPlan attn_fwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int 
 
 template <class T, int DP, int OG> static void attn_fwd_og(const AttnFwd& a, hipStream_t stream) {
     if (!a.units) {
-        attn_fwd_kernel<T, DP, OG><<<attn_grid(a.d, a.ntile), 256, 0, stream>>>(a);
+        attn_fwd_kernel<T, DP, OG><<<(unsigned)attn_grid(a.d, a.ntile), 256, 0, stream>>>(a);
         return;
     }
     attn_fwd_kernel<T, DP, OG><<<dim3(a.d.Hkv * a.ntile, a.units), 256, 0, stream>>>(a);
@@ -400,6 +400,7 @@ int attn_check(const PpvAttention* x, AttnDims* d) {
         x->D % v || !(x->scale > 0.f) || x->scale > 1e30f)
         return PPV_ERR_BAD_SIZE;
     if ((long)x->Tq * (x->H / x->Hkv) > 0x3fffffffL || x->Tk > 0x3fffffff || (long)x->B * x->Hkv > 0x3fffffffL) return PPV_ERR_BAD_SIZE;
+    if ((long)x->B * ((x->Tk + 31L) / 32) > 0x3fffffffL) return PPV_ERR_BAD_SIZE;              // (key tiles of all sequences are counted in 32 bits)
     const long st[] = {x->sqb, x->sqt, x->sqh, x->skb, x->skt, x->skh, x->svb, x->svt, x->svh};
     for (long s : st)
         if (s < 0 || s % v) return PPV_ERR_BAD_SIZE;
@@ -430,7 +431,7 @@ int ppv_attention_fwd(const PpvAttention* x, ppv_stream_t stream) {
     if (int e = attn_check(x, &a.d)) return e;
     const AttnPlan p = attn_fwd_plan(x->B, x->Hkv, a.d.G, x->Tq, x->Tk, x->D, x->dtype == 0 ? 4 : 2);
     if (p.units && !x->workspace) return PPV_ERR_WORKSPACE;
-    if ((size_t)a.d.nbh * p.ntile > 0x7ffffff0u) return PPV_ERR_BAD_SIZE;
+    if (attn_grid(a.d, p.ntile) > ATTN_MAX_GRID || (p.units && (size_t)x->workspace % 16)) return PPV_ERR_BAD_SIZE;
     a.q = {x->q, x->sqb, x->sqt, x->sqh};
     a.k = {x->k, x->skb, x->skt, x->skh};
     a.v = {x->v, x->svb, x->svt, x->svh};

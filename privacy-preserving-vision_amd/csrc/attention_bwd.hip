@@ -438,13 +438,13 @@ static BwdPlan attn_bwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int e
 template <class T, int DP> static int attn_bwd_t(AttnBwd a, const BwdPlan& p, hipStream_t stream) {
     constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;
     const AttnDims& d = a.d;
-    if ((long)d.nbh * p.tq > 0x7ffffff0L || (long)d.nbh * p.tk > 0x7ffffff0L) return PPV_ERR_BAD_SIZE;
+    if (attn_grid(d, p.tq) > ATTN_MAX_GRID || attn_grid(d, p.tk) > ATTN_MAX_GRID) return PPV_ERR_BAD_SIZE;
     auto sum = [&](const float* part, void* out, int nsplit, int G, int n) {
         attn_split_sum_kernel<T, DP><<<(unsigned)(((long)d.nbh * n * (DP / 4) + 255) / 256), 256, 0, stream>>>(part, (T*)out, nsplit, d.nbh, d.Hkv, G, n, d.D);
     };
     a.ntile = p.tq;
     a.nsplit = p.sq;
-    dim3 grid(attn_grid(d, p.tq), p.sq);
+    dim3 grid((unsigned)attn_grid(d, p.tq), p.sq);
     if (p.nq == 1) attn_dq_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
     else if (p.nq == 2) attn_dq_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dq_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);
@@ -452,7 +452,7 @@ template <class T, int DP> static int attn_bwd_t(AttnBwd a, const BwdPlan& p, hi
     if (d.Tk == 0) return ppv_last_error();
     a.ntile = p.tk;
     a.nsplit = p.sk;
-    grid = dim3(attn_grid(d, p.tk), p.sk);
+    grid = dim3((unsigned)attn_grid(d, p.tk), p.sk);
     if (p.nk == 1) attn_dkv_kernel<T, DP, LEAST><<<grid, 256, 0, stream>>>(a);
     else if (p.nk == 2) attn_dkv_kernel<T, DP, 2><<<grid, 256, 0, stream>>>(a);
     else attn_dkv_kernel<T, DP, 4><<<grid, 256, 0, stream>>>(a);

@@ -130,7 +130,8 @@ __device__ __forceinline__ bool attn_block(const AttnDims& d, int ntile, int& bh
     bh = h * lanes + (d.xcd ? blockIdx.x & 7 : 0);
     return bh < d.nbh;
 }
-static inline unsigned attn_grid(const AttnDims& d, int ntile) { return (unsigned)((d.xcd ? (d.nbh + 7) / 8 * 8 : d.nbh) * (long)ntile); }
+static inline long attn_grid(const AttnDims& d, int ntile) { return (d.xcd ? (d.nbh + 7) / 8 * 8 : d.nbh) * (long)ntile; }
+constexpr long ATTN_MAX_GRID = (1 << 24) - 1;                  // workgroups of 256: a launch counts its work items in 32 bits
 
 __device__ __forceinline__ float half_swap_max(float v) {
     auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);

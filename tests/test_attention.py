@@ -357,3 +357,24 @@ def test_attention_is_differentiable_once_and_keeps_what_it_needs():
     lens.fill_(9)                                                  # lengths are operands: changed under a pending backward pass, they are refused
     with pytest.raises(RuntimeError):
         out.sum().backward()
+
+
+def test_attention_entry_points_refuse_more_than_a_launch_holds():
+    """Workgroups beyond 2^24 (work items are counted in 32 bits), key tiles beyond 2^30, a workspace off 16 bytes: refused before anything is launched."""
+    from ppv_amd import _lib
+    L = _lib.lib()
+
+    def args(**kw):
+        a = _lib.Attention()
+        for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "workspace"):
+            setattr(a, n, 64)
+        a.B, a.H, a.Hkv, a.Tq, a.Tk, a.D, a.dtype, a.causal, a.scale = 1, 1, 1, 1, 1, 8, 1, 0, 1.0
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return a
+
+    for kw in ({"B": 1 << 24}, {"B": (1 << 24) - 7}, {"B": 1 << 20, "Tq": 2048}, {"B": 200, "Tk": 1 << 28}):
+        assert L.ppv_attention_fwd(args(**kw), None) == _lib.PPV_ERR_BAD_SIZE, kw
+        assert L.ppv_attention_bwd(args(**kw), None) == _lib.PPV_ERR_BAD_SIZE, kw
+    assert L.ppv_attention_bwd(args(B=1 << 20, Tk=2048), None) == _lib.PPV_ERR_BAD_SIZE
+    assert L.ppv_attention_fwd(args(Tk=100000, workspace=72), None) == _lib.PPV_ERR_BAD_SIZE
