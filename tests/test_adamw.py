@@ -339,3 +339,15 @@ def test_adamw_refuses_parameters_that_share_memory():
         AdamW([c, a, b]).step()
     AdamW([c, a], lr=0.5, weight_decay=0.0).step()              # neighbours
     assert (x + 0.5).abs().max() < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_a_tensor_beyond_32_bits(bits):
+    from ppv_amd.optim import AdamW
+    n = (1 << 32) + 4099
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    p.grad = torch.ones(n, device="cuda")
+    AdamW([p], lr=0.5, weight_decay=0.0, state_bits=bits).step()
+    lo, hi = p.detach().aminmax()
+    assert lo == hi and abs(float(lo) + 0.5) < 1e-6

@@ -378,3 +378,29 @@ def test_attention_entry_points_refuse_more_than_a_launch_holds():
         assert L.ppv_attention_bwd(args(**kw), None) == _lib.PPV_ERR_BAD_SIZE, kw
     assert L.ppv_attention_bwd(args(B=1 << 20, Tk=2048), None) == _lib.PPV_ERR_BAD_SIZE
     assert L.ppv_attention_fwd(args(Tk=100000, workspace=72), None) == _lib.PPV_ERR_BAD_SIZE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Tq", [1, 130])
+def test_attention_reads_a_cache_whose_offsets_pass_32_bits(Tq, dt):
+    """A cache [T, layers * heads * D ...] read in place through its token stride: the same bits as from a packed copy."""
+    from ppv_amd.attention import multihead_attention
+    T, D, step = 4200, 64, 1 << 20                              # offsets up to 4.4e9 elements
+    store = torch.empty(T * step, dtype=dt, device="cuda")
+    gen = torch.Generator().manual_seed(7)
+    wide = store.view(1, T, step)
+    k, v = wide[..., :2 * D].unflatten(2, (2, D)), wide[..., step - 2 * D:].unflatten(2, (2, D))
+    packed = [torch.randn(1, T, 2, D, generator=gen).to(dt).cuda() for _ in range(2)]
+    k.copy_(packed[0])
+    v.copy_(packed[1])
+    assert (k.stride(1), v.stride(1)) == (step, step)
+    q, g = (torch.randn(1, Tq, 4, D, generator=gen).to(dt).cuda() for _ in range(2))
+    runs = []
+    for a, b in ((k, v), packed):
+        leaves = [t.detach().requires_grad_(True) for t in (q, a, b)]
+        out = multihead_attention(*leaves, causal=True)
+        runs.append((out,) + torch.autograd.grad(out, leaves, g))
+    assert all(torch.equal(x, y) for x, y in zip(*runs))
+    far = wide[:, ::8, :2 * D].unflatten(2, (2, D))            # a token stride of 2^23: copied
+    assert torch.equal(multihead_attention(q, far, far), multihead_attention(q, far.contiguous(), far.contiguous()))

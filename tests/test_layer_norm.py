@@ -262,3 +262,18 @@ def test_captured_backward_over_a_living_eager_graph_is_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(dx, want[0]) and eager.requires_grad
+
+
+@pytest.mark.gpu
+def test_layer_norm_of_rows_whose_offsets_pass_32_bits():
+    from ppv_amd.nn_ops import layer_norm
+    rows, C, step = 4200, 200, 1 << 20                          # offsets up to 4.4e9 elements
+    x, w, b, dy = (t.cuda() for t in _case(rows, C, torch.bfloat16, torch.float32, 3))
+    far = torch.empty(rows * step, dtype=torch.bfloat16, device="cuda").view(rows, step)[:, 5:5 + C]
+    far.copy_(x)
+    runs = []
+    for t in (far, x):
+        leaf = t.detach().requires_grad_(True)
+        y = layer_norm(leaf, w, b)
+        runs.append((y,) + torch.autograd.grad(y, leaf, dy))
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
