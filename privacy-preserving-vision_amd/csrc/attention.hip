@@ -69,7 +69,7 @@ template <class T, int DP, int OG> struct FwdShape {
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 81920 ? 2 : 1;                 // tile buffers
     static constexpr int PARK = (SG - 1) * OG * (DP / 2 + 2) * 256;                        // where the key groups meet
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
-    static constexpr int WAVES = DP == 128 && sizeof(T) == 4 ? 1 : 2;         // per SIMD: 512 or 256 registers
+    static constexpr int WAVES = DP > 64 && sizeof(T) == 4 ? 1 : 2;         // per SIMD: 512 or 256 registers
 };
 
 template <class T, int DP, int OG>
@@ -362,7 +362,7 @@ struct AttnPlan { int og, ntile, dp; long units; };
 static AttnPlan attn_fwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int es) {
     AttnPlan p;
     const long rows = (long)Tq * G;
-    p.dp = D <= 32 ? 32 : D <= 64 ? 64 : 128;
+    p.dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
     p.og = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
     p.ntile = (int)((rows + p.og * 32 - 1) / (p.og * 32));
     // split where the tiles alone leave the chip idle: at most 512 workgroups (two for each CU, all of them resident: with 544 the last
@@ -389,7 +389,8 @@ template <class T, int DP> static int attn_fwd_t(const AttnFwd& a, const AttnPla
     return ppv_last_error();
 }
 template <class T> static int attn_fwd_dp(const AttnFwd& a, const AttnPlan& p, hipStream_t stream) {
-    return p.dp == 32 ? attn_fwd_t<T, 32>(a, p, stream) : p.dp == 64 ? attn_fwd_t<T, 64>(a, p, stream) : attn_fwd_t<T, 128>(a, p, stream);
+    return p.dp == 32 ? attn_fwd_t<T, 32>(a, p, stream) : p.dp == 64 ? attn_fwd_t<T, 64>(a, p, stream)
+         : p.dp == 96 ? attn_fwd_t<T, 96>(a, p, stream) : attn_fwd_t<T, 128>(a, p, stream);
 }
 
 // the checks that both directions share; 0 or an error

@@ -42,7 +42,7 @@ template <class T, int DP, int OG, int ACC> struct BwdShape {
     static constexpr int NB = 4 * Tile<T, DP>::bytes(KT) <= 81920 ? 2 : 1;
     static constexpr int PARK = (SG - 1) * OG * (DP / 2) * 256 * ACC;
     static constexpr int LDS = 2 * NB * Tile<T, DP>::bytes(KT) > PARK ? 2 * NB * Tile<T, DP>::bytes(KT) : PARK;
-    static constexpr int WAVES = DP == 128 && (sizeof(T) == 4 || OG < ACC * 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
+    static constexpr int WAVES = DP > 64 && (sizeof(T) == 4 || OG < ACC * 2) ? 1 : DP == 64 && sizeof(T) == 4 && OG <= ACC ? 1 : 2;
 };
 // adds the other groups' accumulators to the first one's (in their order); false: this wave is done
 template <int DB, int OG, int SG> __device__ __forceinline__ bool meet(f32x16* acc, float* lds, int og, int sg, int lane) {
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     constexpr int NT = 256, QT = SH::KT, NB = SH::NB, SG = SH::SG;
     // K, V, dK, dV of 128 in registers leave one wave per SIMD (328 registers: 430 us where this form took 363, 2 x 16 heads of 4096
     // tokens, causal): V waits in LDS instead
-    constexpr bool VL = DP == 128 && sizeof(T) == 2;
+    constexpr bool VL = DP > 64 && sizeof(T) == 2;
     __shared__ __attribute__((aligned(16))) char smem[SH::LDS];
     __shared__ __attribute__((aligned(16))) char vown[VL ? TL::bytes(OG * 32) : 16];
     __shared__ __attribute__((aligned(16))) float stat[NB][2][QT];     // lse, delta
@@ -413,8 +413,8 @@ template <class T, int DP> __global__ __launch_bounds__(256) void attn_split_sum
 struct BwdPlan { int nq, nk, tq, tk, sq, sk, dp; size_t part; };
 static BwdPlan attn_bwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int es) {
     BwdPlan p;
-    p.dp = D <= 32 ? 32 : D <= 64 ? 64 : 128;
-    const int least = es == 4 && p.dp == 128 ? 2 : 1;          // (one group that holds a row's or a key's part of 128 f32 spills)
+    p.dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
+    const int least = es == 4 && p.dp > 64 ? 2 : 1;            // (one group that holds a row's or a key's part of 128 f32 spills)
     auto groups = [&](long n) { return n <= 32 && least == 1 ? 1 : n <= 64 ? 2 : 4; };
     const long rows = (long)Tq * G, bh = (long)B * Hkv;
     p.nq = groups(rows);
@@ -436,7 +436,7 @@ static BwdPlan attn_bwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int e
 }
 
 template <class T, int DP> static int attn_bwd_t(AttnBwd a, const BwdPlan& p, hipStream_t stream) {
-    constexpr int LEAST = sizeof(T) == 4 && DP == 128 ? 2 : 1;
+    constexpr int LEAST = sizeof(T) == 4 && DP > 64 ? 2 : 1;
     const AttnDims& d = a.d;
     if (attn_grid(d, p.tq) > ATTN_MAX_GRID || attn_grid(d, p.tk) > ATTN_MAX_GRID) return PPV_ERR_BAD_SIZE;
     auto sum = [&](const float* part, void* out, int nsplit, int G, int n) {
@@ -463,7 +463,8 @@ template <class T, int DP> static int attn_bwd_t(AttnBwd a, const BwdPlan& p, hi
     return ppv_last_error();
 }
 template <class T> static int attn_bwd_dp(const AttnBwd& a, const BwdPlan& p, hipStream_t stream) {
-    return p.dp == 32 ? attn_bwd_t<T, 32>(a, p, stream) : p.dp == 64 ? attn_bwd_t<T, 64>(a, p, stream) : attn_bwd_t<T, 128>(a, p, stream);
+    return p.dp == 32 ? attn_bwd_t<T, 32>(a, p, stream) : p.dp == 64 ? attn_bwd_t<T, 64>(a, p, stream)
+         : p.dp == 96 ? attn_bwd_t<T, 96>(a, p, stream) : attn_bwd_t<T, 128>(a, p, stream);
 }
 
 }  // namespace ppv

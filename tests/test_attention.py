@@ -404,3 +404,16 @@ def test_attention_reads_a_cache_whose_offsets_pass_32_bits(Tq, dt):
     assert all(torch.equal(x, y) for x, y in zip(*runs))
     far = wide[:, ::8, :2 * D].unflatten(2, (2, D))            # a token stride of 2^23: copied
     assert torch.equal(multihead_attention(q, far, far), multihead_attention(q, far.contiguous(), far.contiguous()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hkv,D", [(2, 1, 3001, 8, 2, 80), (1, 40, 1500, 1, 1, 96), (1, 900, 40, 4, 1, 88), (1, 300, 300, 2, 2, 96),
+                                             (4, 52, 130, 8, 4, 80), (64, 130, 70, 4, 4, 72)])
+def test_attention_of_head_dimensions_between_64_and_96(B, Tq, Tk, H, Hkv, D, causal, dt):
+    """Staged in rows of 128, multiplied as 96: with the keys split, the backward walks split, neither, and whole tiles of every direction."""
+    q, k, v, g = _inputs(B, Tq, Tk, H, Hkv, D, DT[dt], Tq + D)
+    k_lens = torch.tensor([max(0, Tk - 5 * b) for b in range(B)], dtype=torch.int32)
+    want, tol = _bounds(q, k, v, g, causal, None, k_lens, None)
+    _check(NAMES, _run(q, k, v, g, causal=causal, k_lens=k_lens), want, tol)
