@@ -297,7 +297,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
 // A list of parameters with their moments (ms, vs undefined: 32 bits) whose gradients are taken as they are at each step.  The descriptor table on
 // the device is made again whenever one of the addresses it holds, or the stream, is another one.
 struct AdamWList {
-    std::vector<Tensor> p, m, v, ms, vs;
+    std::vector<Tensor> p, m, v, ms, vs, rest;                 // rest: the group's parameters that had no gradient
     std::vector<int64_t> place, key;
     Tensor table;
     int records = 0, blocks = 0;
@@ -307,6 +307,15 @@ struct AdamWList {
         : p(std::move(p_)), m(std::move(m_)), v(std::move(v_)), place(std::move(place_)) {
         for (const auto& t : ms_) ms.push_back(t.value_or(Tensor()));
         for (const auto& t : vs_) vs.push_back(t.value_or(Tensor()));
+    }
+
+    // every parameter of the list has a gradient, none of the others has
+    bool complete() const {
+        for (const auto& t : p)
+            if (!t.grad().defined()) return false;
+        for (const auto& t : rest)
+            if (t.grad().defined()) return false;
+        return true;
     }
 
     void step(double lr, double b1, double b2, double eps, double wd, double number, uint32_t seed) {
@@ -342,6 +351,14 @@ struct AdamWList {
         auto* r = static_cast<Record*>(host.data_ptr());
         for (size_t i = 0; i < p.size(); ++i) {
             const int64_t* at = now.data() + 1 + i * 7;
+            auto fits = [&](const Tensor& t, at::ScalarType kind, int64_t n) {
+                return t.scalar_type() == kind && t.numel() == n && t.is_contiguous() && t.device() == p[i].device();
+            };
+            const bool small = ms[i].defined();                // (`.data` of a tensor that is kept may have become another one)
+            const auto kind = small ? at::kFloat8_e4m3fn : at::kFloat;
+            TORCH_CHECK_VALUE(fits(m[i], kind, at[6]) && fits(v[i], kind, at[6]) &&
+                                  (!small || (fits(ms[i], at::kFloat, (at[6] + 255) / 256) && fits(vs[i], at::kFloat, (at[6] + 255) / 256))),
+                              "ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)");
             if (at[6] == 0) continue;
             Record& x = r[records++];
             std::copy(at, at + 6, x.at);
@@ -368,5 +385,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
     py::class_<AdamWList>(mod, "AdamWList")
         .def(py::init<std::vector<Tensor>, std::vector<Tensor>, std::vector<Tensor>, const std::vector<std::optional<Tensor>>&,
                       const std::vector<std::optional<Tensor>>&, std::vector<int64_t>>())
+        .def("without", [](AdamWList& a, std::vector<Tensor> rest) { a.rest = std::move(rest); })
+        .def("complete", &AdamWList::complete)
         .def("step", &AdamWList::step, release());
 }

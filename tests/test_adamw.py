@@ -351,3 +351,58 @@ def test_adamw_of_a_tensor_beyond_32_bits(bits):
     AdamW([p], lr=0.5, weight_decay=0.0, state_bits=bits).step()
     lo, hi = p.detach().aminmax()
     assert lo == hi and abs(float(lo) + 0.5) < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps_that_start_from_the_last_one_are_those_that_do_not(bits):
+    """A step that finds everything as the last one left it goes a shorter way: the same bits as an optimiser that forgets, whatever is changed in between:
+    a gradient that is missing or comes, a replaced moment or state, a changed number, a new group, other memory behind a parameter."""
+    from ppv_amd.optim import AdamW
+    gen = torch.Generator().manual_seed(3)
+    first = [torch.randn(n, generator=gen) for n in (300, 5, 5000, 64)]
+    grads = [[torch.randn(len(t), generator=gen) for t in first] for _ in range(12)]
+
+    def run(forget):
+        ps = [torch.nn.Parameter(t.clone().cuda()) for t in first]
+        o = AdamW(ps[:3], lr=1e-2, state_bits=bits, seed=5)
+        for k in range(12):
+            for p, g in zip(ps, grads[k]):
+                p.grad = g.cuda()
+            if k in (3, 4):
+                ps[1].grad = None                               # its count stays behind: two launches from here on
+            if k == 6:
+                o.state[ps[1]]["step"] = o.state[ps[0]]["step"] # one again
+            if k == 7:
+                o.state[ps[0]]["exp_avg"] = o.state[ps[0]]["exp_avg"].clone()
+                o.state[ps[0]][list(o.state[ps[0]])[1]].copy_(o.state[ps[0]]["exp_avg"])
+            if k == 8:
+                o.state[ps[2]] = {n: (t.clone() if torch.is_tensor(t) else t) for n, t in o.state[ps[2]].items()}
+                o.add_param_group({"params": [ps[3]], "lr": 1e-3})
+            if k == 9:
+                ps[0].data = ps[0].data.clone()
+                o.param_groups[0]["lr"] = 3e-3
+            if k == 10:
+                del o.param_groups[0]["params"][1]
+                for st in (o.state[ps[0]], o.state[ps[2]]):
+                    st["step"] = 20.0
+            if forget:
+                o._last.clear()
+                o._tables.clear()
+            o.step()
+        return [p.detach() for p in ps] + [t for p in ps for t in o.state[p].values()]
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) if torch.is_tensor(a) else a == b
+
+
+@pytest.mark.gpu
+def test_adamw_refuses_a_state_whose_memory_was_swapped():
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(64, device="cuda"))
+    p.grad = torch.ones(64, device="cuda")
+    o = AdamW([p])
+    o.step()
+    o.state[p]["exp_avg_sq"].data = torch.zeros(3, device="cuda")
+    with pytest.raises(ValueError):
+        o.step()
