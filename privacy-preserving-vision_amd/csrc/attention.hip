@@ -11,8 +11,9 @@
 //   * rows behind a sequence's end and rows that see no key are zeros, with -inf; keys behind the end are not read;
 //   * few rows: the keys are split over workgroups in units of equal length whatever the sequences' lengths, each leaves (O, m, l) in f32,
 //     a second launch joins them.
-// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: 160 us = 860 TFLOP/s (a large library product: 1242); one token of 32 heads on
-// 8 key heads of 128 against 4 ragged histories of up to 65536: 772 MB in 140 us = 5.5 TB/s, and 6 us for the join; 32 x 52 rows against 1296
+// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: 155 us = 885 TFLOP/s (a large library product: 1242); the matrix pipe is busy
+// 39 % of the cycles, the vector ALU 40 %, and they hardly overlap (the next tile's scores made while this one's softmax runs: 163 us and more); one token of 32 heads on
+// 8 key heads of 128 against 4 ragged histories of up to 65536: 772 MB in 140-150 us = 5.5-5.1 TB/s, and 6 us for the join; 32 x 52 rows against 1296
 // f32 keys, 8 heads of 64: 61 us, the f32 matrix pipe busy 60 % of them.
 #include "attention_tiles.h"
 

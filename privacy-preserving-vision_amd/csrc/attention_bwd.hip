@@ -11,8 +11,8 @@
 // That is 7 products where one launch with atomics on dQ would need 5.  Where few rows (keys) leave the chip idle, the axis that is walked over is
 // split; the splits' f32 sums are added in their order by a small launch.  Bound by the matrix pipe and, behind it, the LDS: every operand of a
 // tile is read along its rows (S, dP) and across them (dQ, dK, dV).
-// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: dQ 205-215 us = 1000 TFLOP/s, dK / dV 295 us = 930; f32, 32 x 52 rows against
-// 1296 keys, 8 heads of 64: 78 and 136 us, the f32 matrix pipe busy 71 and 61 %.
+// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: dQ 215 us = 960 TFLOP/s, dK / dV 290 us = 945; f32, 32 x 52 rows against
+// 1296 keys, 8 heads of 64: 80 and 137 us, the f32 matrix pipe busy 71 and 61 %.
 #include "attention_tiles.h"
 
 namespace ppv {
