@@ -339,7 +339,16 @@ struct AdamWList {
             describe(now);
             key = std::move(now);
         }
-        if (records) check(abi.adamw_multi(table.data_ptr(), records, blocks, lr, b1, b2, eps, wd, number, seed, st), "ppv_adamw_multi");
+        if (!records) return;
+        check(abi.adamw_multi(table.data_ptr(), records, blocks, lr, b1, b2, eps, wd, number, seed, st), "ppv_adamw_multi");
+        for (const auto* list : {&p, &m, &v, &ms, &vs})
+            for (const Tensor& t : *list) written(t);
+    }
+
+    // The kernel writes through addresses.  What goes by a tensor's version has to be told: autograd's check of saved tensors, and every cache
+    // of a weight's layout (nn_ops._layouts: the convolutions would stay with the weights of the first step).  (Inference tensors have no version.)
+    static void written(const Tensor& t) {
+        if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
 
     void describe(const std::vector<int64_t>& now) {

@@ -406,3 +406,66 @@ def test_adamw_refuses_a_state_whose_memory_was_swapped():
     o.state[p]["exp_avg_sq"].data = torch.zeros(3, device="cuda")
     with pytest.raises(ValueError):
         o.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_raises_the_version_of_what_it_writes(bits):
+    """Parameters and moments are written through their addresses; autograd's check of saved tensors and every cache of a weight's layout go by the
+    version counter.  The short way of a step counts too; what a step does not write keeps its version."""
+    from ppv_amd.optim import AdamW
+    ps = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, [(300,), (64, 128), (5,), (0,)])]
+    opt = AdamW(ps, lr=1e-2, state_bits=bits)
+    for step in range(4):
+        for p in ps[:2] + ps[3:]:
+            p.grad = torch.ones_like(p)
+        was = [p._version for p in ps]
+        held = [(t, t._version) for p in ps for t in opt.state[p].values() if torch.is_tensor(t)] if step else []
+        opt.step()
+        assert ps[0]._version > was[0] and ps[1]._version > was[1] and ps[2]._version == was[2]
+        assert all(t._version > v for t, v in held if t.numel()) and all(p.grad is None or p.grad._version == 0 for p in ps)
+        assert len(held) == (0 if step == 0 else 2 + 2 + (4 if bits == 8 else 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_modules_follow_adamw(bits):
+    """Two steps on a block whose convolutions keep their weights' layouts: value and gradients are those of a new block with the same weights."""
+    from ppv_amd.optim import AdamW
+    from ppv_amd.stargan_blocks import ResBlk
+    torch.manual_seed(0)
+    blk = ResBlk(64, 128, normalize=True, downsample=True).cuda()
+    x = torch.randn(2, 64, 16, 16, device="cuda", requires_grad=True)
+    opt = AdamW(blk.parameters(), lr=3e-2, state_bits=bits, min_8bit_size=256)
+    seen = []
+    for step in range(3):
+        out = blk(x)
+        new = copy.deepcopy(blk)                                # its parameters are other tensors: no layout of theirs is kept
+        for q in new.parameters():
+            q.grad = None
+        want = new(x)
+        assert torch.equal(out, want), step
+        assert all(not torch.equal(out, s) for s in seen)
+        seen.append(out.detach())
+        g = torch.autograd.grad(out.square().sum(), [x] + list(blk.parameters()))
+        h = torch.autograd.grad(want.square().sum(), [x] + list(new.parameters()))
+        assert all(torch.equal(a, b) for a, b in zip(g, h)), step
+        for p, d in zip(blk.parameters(), g[1:]):
+            p.grad = d
+        opt.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_between_forward_and_backward_is_an_error(bits):
+    """The backward pass would mix the weights of two steps."""
+    from ppv_amd.nn_ops import layer_norm
+    from ppv_amd.optim import AdamW
+    x, w = torch.randn(6, 512, device="cuda", requires_grad=True), torch.nn.Parameter(torch.ones(512, device="cuda"))
+    opt = AdamW([w], lr=1e-2, state_bits=bits, min_8bit_size=256)
+    for _ in range(2):
+        w.grad = torch.ones_like(w)
+        y = layer_norm(x, w)
+        opt.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
