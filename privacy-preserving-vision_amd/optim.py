@@ -94,6 +94,8 @@ class Adam(torch.optim.Optimizer):
                 n = t + 1.0
                 _lib.check(L.ppv_adam_multi(desc.data_ptr(), len(sub), blocks, group["lr"], b1, b2, group["eps"], group["weight_decay"],
                                             1.0 - b1 ** n, 1.0 - b2 ** n, _lib.stream_ptr()), "ppv_adam_multi")
+                # (written through addresses: autograd's check of saved tensors and the caches of weight layouts go by the version)
+                torch.autograd.graph.increment_version([t for p in sub for t in (p, self.state[p]["exp_avg"], self.state[p]["exp_avg_sq"])])
                 for p in sub:
                     self.state[p]["step"] += 1
         return loss

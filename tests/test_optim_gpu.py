@@ -117,3 +117,30 @@ def test_adam_follows_a_reloaded_state_and_does_not_grow_its_tables():
         assert torch.allclose(a["exp_avg"], b["exp_avg"].cpu(), rtol=2e-5, atol=1e-7)
         assert torch.allclose(a["exp_avg_sq"], b["exp_avg_sq"].cpu(), rtol=2e-5, atol=1e-9)
     assert len(o_got._tables) == n_tables <= 3                                   # (group, slot) keys are reused: no growth with the step count
+
+
+def test_adam_raises_the_version_of_what_it_writes_and_modules_follow_it():
+    """Adam's kernel writes through addresses: autograd and the convolutions' kept layouts go by the version counter."""
+    import copy
+    from ppv_amd.optim import Adam
+    from ppv_amd.stargan_blocks import ResBlk
+    torch.manual_seed(0)
+    blk = ResBlk(64, 64).cuda()
+    x = torch.randn(2, 64, 16, 16, device="cuda")
+    o = Adam(blk.parameters(), lr=3e-2)
+    for step in range(3):
+        out, want = blk(x), copy.deepcopy(blk)(x)
+        assert torch.equal(out, want), step
+        for p, d in zip(blk.parameters(), torch.autograd.grad(out.square().sum(), list(blk.parameters()))):
+            p.grad = d
+        held = [t for p in blk.parameters() for t in (p, *o.state[p].values()) if torch.is_tensor(t)]
+        was = [t._version for t in held]
+        o.step()
+        assert all(t._version > v for t, v in zip(held, was)), step
+        assert all(p.grad._version == 0 for p in blk.parameters())
+    out = blk(x)
+    for p in blk.parameters():
+        p.grad = torch.zeros_like(p)
+    o.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
