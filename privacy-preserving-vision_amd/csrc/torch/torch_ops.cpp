@@ -6,6 +6,7 @@
 // optim.AdamW); here is what happens after that.  The library's entry points come from the loaded libppv_hip.so by address (bind), so that
 // there is one copy of it.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -58,6 +59,16 @@ ppv_stream_t stream() { return reinterpret_cast<ppv_stream_t>(c10::hip::getCurre
 int code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
 
 template <class P> P* data(const Tensor& t) { return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr; }
+
+// The kernels go by addresses, out of sight of torch's dispatcher.  What it does besides computing would be missing from the result without a word;
+// the arguments of both operators, and the gradients that come back to them, are looked over for it: forward-mode tangents.
+void refuse_unseen(const char* name, std::initializer_list<const Tensor*> ts) {
+    const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor* t : ts) {
+        if (!t->defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!tangents || !t->_fw_grad(0).defined(), "ppv_amd ", name, ": forward-mode derivatives are not implemented");
+    }
+}
 
 // Gradients of a node that is differentiable once: where a graph of the backward pass is asked for, differentiating through it is an error.
 variable_list once(variable_list grads) {
@@ -132,6 +143,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         variable_list r;
         {
             at::NoGradGuard off;
+            refuse_unseen("layer_norm", {&grads[0]});
             refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
             const Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2], &g = grads[0];
@@ -170,6 +182,7 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    refuse_unseen("layer_norm", {&x, &w, &b});
     if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
     at::NoGradGuard off;
     c10::DeviceGuard guard(x.device());
@@ -257,6 +270,7 @@ struct Attention : torch::autograd::Function<Attention> {
         variable_list r(7);
         {
             at::NoGradGuard off;
+            refuse_unseen("multihead_attention", {&grads[0]});
             refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
             const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3];
@@ -285,8 +299,9 @@ struct Attention : torch::autograd::Function<Attention> {
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& q_lens, const std::optional<Tensor>& k_lens,
                  bool causal, double scale) {
-    if (wants_grad({&q, &k, &v})) return Attention::apply(q, k, v, q_lens, k_lens, causal, scale);
     const Tensor ql = q_lens.value_or(Tensor()), kl = k_lens.value_or(Tensor());
+    refuse_unseen("multihead_attention", {&q, &k, &v, &ql, &kl});
+    if (wants_grad({&q, &k, &v})) return Attention::apply(q, k, v, q_lens, k_lens, causal, scale);
     at::NoGradGuard off;
     c10::DeviceGuard guard(q.device());
     return unpadded(attention_forward(q, k, v, ql, kl, causal, scale, false).out, q.size(3));

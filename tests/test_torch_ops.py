@@ -1,0 +1,48 @@
+"""The autograd nodes of lib/ppv_torch.so (csrc/torch/torch_ops.cpp) behind layer_norm and multihead_attention: what torch does with an operator
+besides calling it.  Their kernels go by addresses, so each of these is refused, never left out of the result.  (The refusals come before
+anything else in the native functions: they are tested there without a GPU, and through the public entry points with one.)"""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+
+def _native():
+    from ppv_amd import _lib
+    T = _lib.torch_ops()
+    return (lambda x, w=None, b=None: T.layer_norm(x, w, b, 1e-5)), (lambda q, k, v: T.attention(q, k, v, None, None, False, 0.25))
+
+
+def _public():
+    from ppv_amd.attention import multihead_attention
+    from ppv_amd.nn_ops import layer_norm
+    return layer_norm, multihead_attention
+
+
+WHERE = [("cpu", _native), pytest.param("cuda", _public, marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device,entries", WHERE)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_refused(device, entries, grad):
+    norm, attend = entries()
+    x, w = torch.ones(4, 64, device=device, requires_grad=grad), torch.ones(64, device=device)
+    q = torch.ones(1, 4, 2, 16, device=device, requires_grad=grad)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for call in (lambda: norm(dual(x)), lambda: norm(x, dual(w)), lambda: norm(x, w, dual(w)), lambda: norm(x, None, dual(w)),
+                     lambda: attend(dual(q), q, q), lambda: attend(q, dual(q), q), lambda: attend(q, q, dual(q))):
+            with torch.no_grad() if not grad else torch.enable_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_of_the_gradient_are_refused():
+    """Forward over reverse: a tangent that comes in with the gradient of the result."""
+    norm, attend = _public()
+    x, q = torch.ones(4, 64, device="cuda", requires_grad=True), torch.ones(1, 4, 2, 16, device="cuda", requires_grad=True)
+    for leaf, y in ((x, norm(x)), (q, attend(q, q, q))):
+        with fw.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        with fw.dual_level():                                   # a level without tangents changes nothing
+            want, = torch.autograd.grad((attend(q, q, q) if leaf is q else norm(x)).sum(), leaf)
+        assert torch.isfinite(want).all()
