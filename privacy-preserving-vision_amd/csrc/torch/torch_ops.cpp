@@ -8,6 +8,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/stl.h>
@@ -15,6 +17,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <unordered_set>
@@ -61,8 +64,16 @@ int code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1
 template <class P> P* data(const Tensor& t) { return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr; }
 
 // The kernels go by addresses, out of sight of torch's dispatcher.  What it does besides computing would be missing from the result without a word;
-// the arguments of both operators, and the gradients that come back to them, are looked over for it: forward-mode tangents.
+// the arguments of both operators, and the gradients that come back to them, are looked over for it: forward-mode tangents, and whoever records the
+// dispatched calls to run them again (torch.jit.trace, make_fx) or to run them without data: the record would be the allocation of the result alone.
 void refuse_unseen(const char* name, std::initializer_list<const Tensor*> ts) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "ppv_amd ", name, ": torch.jit.trace does not see the kernel");
+    TORCH_CHECK_NOT_IMPLEMENTED(!TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) &&
+                                    !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL) &&
+                                    !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
+                                "ppv_amd ", name, ": a tracing mode (make_fx, fake tensors, functionalization) does not see the kernel");
     const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Tensor* t : ts) {
         if (!t->defined()) continue;

@@ -46,3 +46,37 @@ def test_forward_mode_tangents_of_the_gradient_are_refused():
         with fw.dual_level():                                   # a level without tangents changes nothing
             want, = torch.autograd.grad((attend(q, q, q) if leaf is q else norm(x)).sum(), leaf)
         assert torch.isfinite(want).all()
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("device,entries", WHERE)
+@pytest.mark.parametrize("grad", [False, True])
+def test_what_records_calls_is_refused(device, entries, grad):
+    """A trace would hold the allocation of the result and nothing else: replayed, whatever lay in that memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    norm, attend = entries()
+    x, q = torch.ones(4, 64, device=device, requires_grad=grad), torch.ones(1, 4, 2, 16, device=device, requires_grad=grad)
+    for call, t in ((lambda a: norm(a), x), (lambda a: attend(a, a, a), q)):
+        with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+            torch.jit.trace(call, (t,), check_trace=False)
+        for pre in (False, True):
+            with pytest.raises(NotImplementedError, match="does not see the kernel"):
+                make_fx(call, pre_dispatch=pre)(t)
+        with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(NotImplementedError, match="does not see the kernel"):
+            call(t)
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_compiled_callers_run_the_operators_themselves():
+    """torch.compile breaks its graph at the operators: the same numbers, value and gradient."""
+    norm, attend = _public()
+    torch.manual_seed(0)
+    x = torch.randn(3, 5, 2, 32, device="cuda", requires_grad=True)
+    f = lambda a: attend(norm(a * 2.0), a, a, causal=True) + 1.0
+    g = torch.compile(f, backend="eager")
+    for _ in range(2):
+        want, got = f(x), g(x)
+        assert torch.equal(want, got)
+        assert torch.equal(*(torch.autograd.grad(y.square().sum(), x)[0] for y in (want, got)))
