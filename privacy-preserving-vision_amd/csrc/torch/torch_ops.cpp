@@ -63,9 +63,17 @@ int code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1
 
 template <class P> P* data(const Tensor& t) { return t.defined() ? static_cast<P*>(t.data_ptr()) : nullptr; }
 
+constexpr c10::DispatchKeySet stand_ins({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::BatchedNestedTensor,
+                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched, c10::DispatchKey::Functionalize});
+
+// A tensor whose memory holds its values: not a negation that is still to be done (z.conj().imag), nor zeros without memory.
+bool is_plain(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
+Tensor plain(const Tensor& t) { return is_plain(t) ? t : t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
+
 // The kernels go by addresses, out of sight of torch's dispatcher.  What it does besides computing would be missing from the result without a word;
 // the arguments of both operators, and the gradients that come back to them, are looked over for it: forward-mode tangents, and whoever records the
-// dispatched calls to run them again (torch.jit.trace, make_fx) or to run them without data: the record would be the allocation of the result alone.
+// dispatched calls to run them again (torch.jit.trace, make_fx) or to run them without data: the record would be the allocation of the result alone;
+// tensors that stand for others (functorch's, subclasses with a dispatch of their own).
 void refuse_unseen(const char* name, std::initializer_list<const Tensor*> ts) {
     using c10::impl::TorchDispatchModeKey;
     using c10::impl::TorchDispatchModeTLS;
@@ -77,6 +85,8 @@ void refuse_unseen(const char* name, std::initializer_list<const Tensor*> ts) {
     const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Tensor* t : ts) {
         if (!t->defined()) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->key_set().has_any(stand_ins), "ppv_amd ", name,
+                                    ": tensors under torch.func / vmap and subclasses with a __torch_dispatch__ do not reach the kernel");
         TORCH_CHECK_NOT_IMPLEMENTED(!tangents || !t->_fw_grad(0).defined(), "ppv_amd ", name, ": forward-mode derivatives are not implemented");
     }
 }
@@ -120,7 +130,8 @@ void refuse_capture_of_eager_graph() {
 // ------------------------------------------------------------------------------------------------------------------------- layer norm
 
 Tensor rows_of(const Tensor& t, int64_t C) {
-    Tensor r = t.dim() == 2 ? t : t.reshape({-1, C});
+    Tensor r = plain(t);
+    if (t.dim() != 2) r = r.reshape({-1, C});
     return C == 1 || r.stride(1) == 1 ? r : r.contiguous();
 }
 long row_stride(const Tensor& r) { return r.size(0) == 1 ? 0 : r.stride(0); }
@@ -142,7 +153,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
         c10::DeviceGuard guard(x.device());
         const Tensor x2 = rows_of(x, x.size(-1));
-        const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+        const Tensor w = weight ? plain(weight->contiguous()) : Tensor(), b = bias ? plain(bias->contiguous()) : Tensor();
         auto [y, stats] = norm_forward(x2, w, b, eps, true);
         ctx->save_for_backward({x2, w, stats});
         const auto& par = w.defined() ? w : b;
@@ -197,7 +208,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
     at::NoGradGuard off;
     c10::DeviceGuard guard(x.device());
-    const Tensor y = norm_forward(rows_of(x, x.size(-1)), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, false).first;
+    const Tensor y = norm_forward(rows_of(x, x.size(-1)), w.defined() ? plain(w.contiguous()) : w, b.defined() ? plain(b.contiguous()) : b, eps, false).first;
     return x.dim() == 2 ? y : y.view(x.sizes());
 }
 
@@ -207,6 +218,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
 // that is already so is taken as it is, any other is copied (zeros behind D add nothing to a product).
 Tensor operand(const Tensor& t, int64_t Dp) {
     const int64_t v = 16 / t.element_size();
+    if (!is_plain(t)) return operand(plain(t), Dp);
     bool fits = t.size(3) == Dp && t.stride(3) == 1 && reinterpret_cast<size_t>(t.data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) == 1 || t.stride(i) % v == 0);
     if (fits && (t.size(1) == 1 || t.stride(1) <= 1 << 22)) return t;
@@ -354,7 +366,7 @@ struct AdamWList {
         for (size_t i = 0; i < p.size(); ++i) {
             const Tensor& g = p[i].grad();
             TORCH_CHECK_NOT_IMPLEMENTED(g.defined() && g.layout() == at::kStrided && g.scalar_type() == at::kFloat && g.is_contiguous() &&
-                                            g.device() == dev && p[i].scalar_type() == at::kFloat && p[i].is_contiguous() && p[i].device() == dev &&
+                                            g.device() == dev && is_plain(g) && is_plain(p[i]) && p[i].scalar_type() == at::kFloat && p[i].is_contiguous() && p[i].device() == dev &&
                                             dev.is_cuda() && g.numel() == p[i].numel(),
                                         "ppv_amd.optim.AdamW: contiguous f32 parameters and gradients on one GPU only");
             const Tensor* held[] = {&p[i], &g, &m[i], &v[i], &ms[i], &vs[i]};

@@ -80,3 +80,49 @@ def test_compiled_callers_run_the_operators_themselves():
         want, got = f(x), g(x)
         assert torch.equal(want, got)
         assert torch.equal(*(torch.autograd.grad(y.square().sum(), x)[0] for y in (want, got)))
+
+
+class _Logged(torch.Tensor):
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("device,entries", WHERE)
+def test_tensors_that_stand_for_others_are_refused(device, entries):
+    norm, attend = entries()
+    x, q = torch.ones(4, 64, device=device), torch.ones(2, 1, 4, 2, 16, device=device)
+    for call in (lambda: torch.vmap(lambda a: norm(a.view(1, 64)))(x), lambda: torch.func.grad(lambda a: norm(a).sum())(x),
+                 lambda: torch.func.jvp(lambda a: norm(a), (x,), (x,)), lambda: torch.vmap(lambda a: attend(a, a, a))(q),
+                 lambda: torch.vmap(lambda a: attend(q[0], a, q[0]))(q), lambda: torch.func.vjp(lambda a: attend(a, a, a), q[0]),
+                 lambda: norm(x.as_subclass(_Logged)), lambda: norm(x, x[0].as_subclass(_Logged)), lambda: attend(q[0], q[0], q[0].as_subclass(_Logged))):
+        with pytest.raises(NotImplementedError, match="do not reach the kernel"):
+            call()
+
+
+@pytest.mark.gpu
+def test_negations_still_to_be_done_are_done():
+    """z.conj().imag and the like are the old memory with a note to negate it: as argument, parameter and gradient."""
+    from ppv_amd.optim import AdamW
+    norm, attend = _public()
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen).cuda()
+    x, w, b, q, k, v = r(5, 64), r(64), r(64), r(1, 5, 2, 16), r(1, 7, 2, 16), r(1, 7, 2, 16)
+    neg = lambda t: torch._neg_view(t)
+    assert neg(x).is_neg() and neg(x).data_ptr() == x.data_ptr()
+    col = torch.complex(r(6, 1), r(6, 1))                       # (one column: every stride fits)
+    for got, want in ((norm(neg(x), neg(w), neg(b)), norm(-x, -w, -b)), (norm(neg(x.view(1, 5, 64))), norm(-x.view(1, 5, 64))),
+                      (attend(neg(q), neg(k), neg(v)), attend(-q, -k, -v)), (norm(x, None, neg(b)), norm(x, None, -b)),
+                      (norm(col.conj().imag, None, b[:1]), norm((-col.imag).clone(), None, b[:1]))):
+        assert torch.equal(got, want)
+    for run in (lambda f: torch.autograd.grad(norm(f(xl), wl), (xl, wl), f(x)), lambda f: torch.autograd.grad(attend(ql, k, v), ql, f(q)),
+                lambda f: torch.autograd.grad(attend(f(ql), k, v), ql, q)):
+        xl, wl, ql = x.clone().requires_grad_(True), w.clone().requires_grad_(True), q.clone().requires_grad_(True)
+        assert all(torch.equal(a, c) for a, c in zip(run(neg), run(lambda t: -t)))
+    zero = torch._efficientzerotensor((5, 64), device="cuda")
+    xl = x.clone().requires_grad_(True)
+    assert torch.equal(norm(zero, w, b), b.expand(5, 64)) and torch.equal(torch.autograd.grad(norm(xl), xl, zero)[0], torch.zeros_like(x))
+    p = torch.nn.Parameter(r(64))
+    p.grad = neg(b)
+    with pytest.raises(NotImplementedError):
+        AdamW([p]).step()
