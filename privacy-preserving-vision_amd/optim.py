@@ -155,6 +155,9 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
+        for group in self.param_groups:        # (a state from before a group had these names)
+            group.setdefault("amsgrad", False)
+            group.setdefault("maximize", False)
         self._number()
 
     def add_param_group(self, param_group):

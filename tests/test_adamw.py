@@ -469,3 +469,16 @@ def test_a_step_between_forward_and_backward_is_an_error(bits):
         opt.step()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+def test_adamw_loads_a_state_that_knows_neither_amsgrad_nor_maximize():
+    """A state written before a group had these names (torch.optim.AdamW fills them in on loading, too)."""
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(4))
+    for drop in (["amsgrad"], ["maximize"], ["amsgrad", "maximize"]):
+        o, sd = AdamW([p]), AdamW([p], lr=0.25).state_dict()
+        for name in drop:
+            del sd["param_groups"][0][name]
+        o.load_state_dict(sd)
+        o.step()                                                # (nothing has a gradient)
+        assert o.param_groups[0]["lr"] == 0.25 and not o.param_groups[0]["amsgrad"] and not o.param_groups[0]["maximize"]
