@@ -105,14 +105,19 @@ __global__ __launch_bounds__(NT) void layernorm_fwd_kernel(const T* __restrict__
     }
 }
 
+// One workgroup for each of n rows (or 16 columns): a launch counts its work items in 32 bits along an axis, so those beyond 2^16 go along y.
+static inline dim3 one_each(long n) { return dim3((unsigned)(n < 65536 ? n : 65536), (unsigned)((n + 65535) / 65536)); }
+__device__ __forceinline__ long which_one() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // rows longer than the registers hold: three passes over the row (the second and third come out of the L2)
 template <class T>
 __global__ __launch_bounds__(256) void layernorm_fwd_long_kernel(const T* __restrict__ x, long ldx, const void* __restrict__ w, const void* __restrict__ b,
                                                                  int wdtype, T* __restrict__ y, float* __restrict__ mean_out,
-                                                                 float* __restrict__ rstd_out, int C, float eps) {
+                                                                 float* __restrict__ rstd_out, long rows, int C, float eps) {
     constexpr int V = 16 / sizeof(T);
     __shared__ float lds[4];
-    const long row = blockIdx.x;
+    const long row = which_one();
+    if (row >= rows) return;
     const T* xr = x + row * ldx;
     float v[V];
     float s = 0.f, q = 0.f;
@@ -291,10 +296,11 @@ __global__ __launch_bounds__(NT, 2) void layernorm_bwd_kernel(const T* __restric
 template <class T>
 __global__ __launch_bounds__(256) void layernorm_bwd_long_kernel(const T* __restrict__ g, long ldg, const T* __restrict__ x, long ldx,
                                                                  const void* __restrict__ w, int wdtype, const float* __restrict__ mean_in,
-                                                                 const float* __restrict__ rstd_in, T* __restrict__ dx, int C) {
+                                                                 const float* __restrict__ rstd_in, T* __restrict__ dx, long rows, int C) {
     constexpr int V = 16 / sizeof(T);
     __shared__ float lds[4];
-    const long row = blockIdx.x;
+    const long row = which_one();
+    if (row >= rows) return;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float s1 = 0.f, s2 = 0.f;
     for (int pass = 0; pass < 2; ++pass) {
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(256) void layernorm_wgrad_reduce_kernel(const float
                                                                      void* __restrict__ db, int wdtype) {
     __shared__ float s[16][17];
     const int j = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const long c = (long)blockIdx.x * 16 + j;                  // over the 2 C columns of a partial row
+    const long c = which_one() * 16 + j;                       // over the 2 C columns of a partial row
     float a = 0.f;
     if (c < 2L * C) {
 #pragma unroll 8
@@ -393,7 +399,7 @@ static int layernorm_fwd_t(const T* x, long ldx, const void* w, const void* b, i
     else if (lpr == 256) LN_FWD(256, 16 / V, 256);
     else if (lpr == 512) LN_FWD(512, 16 / V, 512);
     else if (rows > 0x7fffffffL) return PPV_ERR_BAD_SIZE;
-    else layernorm_fwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, C, eps);
+    else layernorm_fwd_long_kernel<T><<<one_each(rows), 256, 0, stream>>>(x, ldx, w, b, wdtype, y, mean, rstd, rows, C, eps);
 #undef LN_FWD
     return ppv_last_error();
 }
@@ -416,11 +422,11 @@ static int layernorm_bwd_t(const T* g, long ldg, const T* x, long ldx, const voi
     else if (lpr == 512) LN_BWD(512, 16 / V, 512);
     else {
         if (rows > 0x7fffffffL) return PPV_ERR_BAD_SIZE;
-        layernorm_bwd_long_kernel<T><<<(unsigned)rows, 256, 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, C);
+        layernorm_bwd_long_kernel<T><<<one_each(rows), 256, 0, stream>>>(g, ldg, x, ldx, w, wdtype, mean, rstd, dx, rows, C);
         if (part) layernorm_wgrad_long_kernel<T><<<dim3((C + 255) / 256, G), 256, 0, stream>>>(g, ldg, x, ldx, mean, rstd, part, rows, C);
     }
 #undef LN_BWD
-    if (part) layernorm_wgrad_reduce_kernel<<<(unsigned)((2L * C + 15) / 16), 256, 0, stream>>>(part, G, C, dw, db, wdtype);
+    if (part) layernorm_wgrad_reduce_kernel<<<one_each((2L * C + 15) / 16), 256, 0, stream>>>(part, G, C, dw, db, wdtype);
     return ppv_last_error();
 }
 

@@ -277,3 +277,34 @@ def test_layer_norm_of_rows_whose_offsets_pass_32_bits():
         y = layer_norm(leaf, w, b)
         runs.append((y,) + torch.autograd.grad(y, leaf, dy))
     assert all(torch.equal(p, q) for p, q in zip(*runs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,C", [(2, 1 << 27), (70000, 8193)])
+def test_layer_norm_of_more_columns_or_long_rows_than_a_launch_has_along_one_axis(rows, C):
+    """Weight gradients of 2^27 columns (2^28 sums, 16 to a workgroup of 256: 2^32 work items) and 70000 rows that are read in passes.  Rows of +-1 with gradients
+    of small whole numbers: every sum is exact.  The mean is 0 (or 1 / C), h = +-rstd within 2 / C: u / 4 and 3 roundings; a gradient of w adds its
+    rows' products one by one (70000 rows in 64 shares: 1100 additions of at most 2, and 16)."""
+    from ppv_amd.nn_ops import layer_norm
+    i = torch.arange(C, device="cuda")
+    x = (1.0 - 2.0 * (i % 2)).expand(rows, C).contiguous().requires_grad_(True)
+    dy = ((i * 7) % 5 - 2).float()
+    w, b = torch.ones(C, device="cuda", requires_grad=True), torch.zeros(C, device="cuda", requires_grad=True)
+    y = layer_norm(x, w, b, eps=0.0)
+    off = 0.0 if C % 2 == 0 else 4.0 / C
+    assert ((y.detach() - x.detach()).abs().amax()) <= off + 8 * U
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy.expand(rows, C))
+    assert torch.equal(db, dy * rows)
+    assert ((dw - dy * x.detach()[0] * rows).abs() <= rows * 2 * (off + 8 * U) + (0 if rows == 2 else 1116 * U * 2 * rows)).all()
+    s1, s2 = dy.double().mean(), (dy * x.detach()[0]).double().mean()
+    want = dy.double() - s1 - x.detach()[0].double() * s2
+    for r in (0, rows // 2, rows - 1):
+        assert ((dx[r].double() - want).abs() <= 16 * off + 64 * U).all()
+
+
+def test_layer_norm_entry_points_refuse_more_long_rows_than_they_count():
+    import ctypes
+    from ppv_amd import _lib
+    L, p = _lib.lib(), ctypes.c_void_p(64)
+    assert L.ppv_layernorm_fwd(p, 9000, p, p, p, p, p, 1 << 31, 9000, 0, 0, 1e-5, None) == _lib.PPV_ERR_BAD_SIZE
+    assert L.ppv_layernorm_bwd(p, 9000, p, 9000, p, p, p, p, p, p, p, 1 << 31, 9000, 0, 0, None) == _lib.PPV_ERR_BAD_SIZE
