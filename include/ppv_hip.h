@@ -28,6 +28,7 @@ typedef struct ihipStream_t* ppv_stream_t;   /* == hipStream_t */
 #define PPV_ERR_INIT (-1003)
 #define PPV_ERR_WORKSPACE (-1004)
 
+#define PPV_ABI_VERSION 23
 int ppv_abi_version(void);
 int ppv_init(void);
 

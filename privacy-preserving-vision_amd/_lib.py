@@ -260,6 +260,14 @@ _TORCH_ENTRIES = ("ppv_layernorm_fwd", "ppv_layernorm_bwd", "ppv_layernorm_bwd_w
                   "ppv_attention_bwd", "ppv_attention_bwd_workspace_bytes", "ppv_adamw_multi")
 
 
+def _check_torch_ops(mod):
+    """A ppv_torch.so that was compiled against another header or torch would hand over structures of another layout."""
+    built = (getattr(mod, "abi_version", None), getattr(mod, "attention_bytes", None), getattr(mod, "torch_version", None))
+    if built != (ABI_VERSION, ctypes.sizeof(Attention), torch.__version__.split("+")[0]):
+        raise RuntimeError(f"{TORCH_LIB_PATH}: compiled for ABI version {built[0]} (PpvAttention of {built[1]} bytes) and torch {built[2]}, loaded with "
+                           f"ABI version {ABI_VERSION} ({ctypes.sizeof(Attention)} bytes) and torch {torch.__version__} (stale build? re-run __graft_entry__.build())")
+
+
 def torch_ops():
     """lib/ppv_torch.so (csrc/torch/torch_ops.cpp): the autograd nodes in C++, bound to the entry points of the loaded libppv_hip.so."""
     global _torch_ops
@@ -271,6 +279,7 @@ def torch_ops():
         spec = importlib.util.spec_from_file_location("ppv_torch", TORCH_LIB_PATH)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
+        _check_torch_ops(mod)
         mod.bind([(n, ctypes.cast(getattr(L, n), _P).value) for n in _TORCH_ENTRIES])
         _torch_ops = mod
     return _torch_ops

@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
+#include <torch/version.h>
 
 #include <unordered_set>
 
@@ -427,6 +428,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
     namespace py = pybind11;
     using release = py::call_guard<py::gil_scoped_release>;
     mod.def("bind", &bind);
+    // what this file was compiled against: _lib.torch_ops() compares it with what is loaded
+    mod.attr("abi_version") = PPV_ABI_VERSION;
+    mod.attr("attention_bytes") = sizeof(PpvAttention);
+    mod.attr("torch_version") = TORCH_VERSION;
     mod.def("layer_norm", &layer_norm, release());
     mod.def("attention", &attention, release());
     py::class_<AdamWList>(mod, "AdamWList")

@@ -126,3 +126,16 @@ def test_negations_still_to_be_done_are_done():
     p.grad = neg(b)
     with pytest.raises(NotImplementedError):
         AdamW([p]).step()
+
+
+def test_a_library_of_another_build_is_refused():
+    import types
+    from ppv_amd import _lib
+    mod = _lib.torch_ops()
+    names = ("abi_version", "attention_bytes", "torch_version")
+    _lib._check_torch_ops(mod)
+    for name, other in zip(names, (mod.abi_version - 1, mod.attention_bytes + 8, "1.0.0")):
+        with pytest.raises(RuntimeError, match="stale build"):
+            _lib._check_torch_ops(types.SimpleNamespace(**{**{n: getattr(mod, n) for n in names}, name: other}))
+    with pytest.raises(RuntimeError, match="stale build"):
+        _lib._check_torch_ops(types.SimpleNamespace())          # from before it said what it was made for
