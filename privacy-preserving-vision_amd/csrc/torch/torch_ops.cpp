@@ -393,7 +393,7 @@ struct AdamWList {
     void describe(const std::vector<int64_t>& now) {
         struct Record { int64_t at[6], numel; int32_t blk0; uint32_t place; };
         static_assert(sizeof(Record) == 64, "include/ppv_hip.h ppv_adamw_multi");
-        records = 0;
+        int count = 0;                                         // (a list that is refused stays as it was: its key does, too)
         int64_t blk = 0;
         Tensor host = at::empty({(int64_t)(p.size() * sizeof(Record))}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
         auto* r = static_cast<Record*>(host.data_ptr());
@@ -408,7 +408,7 @@ struct AdamWList {
                                   (!small || (fits(ms[i], at::kFloat, (at[6] + 255) / 256) && fits(vs[i], at::kFloat, (at[6] + 255) / 256))),
                               "ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)");
             if (at[6] == 0) continue;
-            Record& x = r[records++];
+            Record& x = r[count++];
             std::copy(at, at + 6, x.at);
             x.numel = at[6];
             x.blk0 = (int32_t)blk;
@@ -416,9 +416,10 @@ struct AdamWList {
             blk += (at[6] + 4095) / 4096;
         }
         TORCH_CHECK(blk <= INT32_MAX, "ppv_amd.optim.AdamW: too many elements in one group");
-        blocks = (int)blk;
         // pinned and non-blocking: a list whose gradients move every step does not wait for the device
-        table = records ? host.to(p[0].device(), at::kByte, /*non_blocking=*/true) : Tensor();
+        table = count ? host.to(p[0].device(), at::kByte, /*non_blocking=*/true) : Tensor();
+        records = count;
+        blocks = (int)blk;
     }
 };
 

@@ -482,3 +482,27 @@ def test_adamw_loads_a_state_that_knows_neither_amsgrad_nor_maximize():
         o.load_state_dict(sd)
         o.step()                                                # (nothing has a gradient)
         assert o.param_groups[0]["lr"] == 0.25 and not o.param_groups[0]["amsgrad"] and not o.param_groups[0]["maximize"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_step_leaves_the_list_as_it_was(bits):
+    """A moment's memory is swapped, the step refused, the memory put back: the next step is the one that would have come."""
+    from ppv_amd.optim import AdamW
+    runs = []
+    for swap in (False, True):
+        ps = [torch.nn.Parameter(t.cuda()) for t in _tensors(0, [(300,), (64, 128), (70,)])]
+        o = AdamW(ps, lr=1e-2, state_bits=bits, min_8bit_size=256)
+        for step in range(3):
+            for p in ps:
+                p.grad = torch.full_like(p, 0.5 + step) if step == 0 else p.grad
+            if swap and step == 2:
+                st = o.state[ps[1]]["exp_avg"]
+                keep = st.data
+                st.data = torch.zeros(3, device="cuda")
+                with pytest.raises(ValueError):
+                    o.step()
+                st.data = keep
+            o.step()
+        runs.append([p.detach() for p in ps])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
