@@ -338,6 +338,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
 struct AdamWList {
     std::vector<Tensor> p, m, v, ms, vs, rest;                 // rest: the group's parameters that had no gradient
     std::vector<int64_t> place, key;
+    static constexpr int WORDS = 11;                           // of the key for each parameter: six addresses, its size, what its moments are
     Tensor table;
     int records = 0, blocks = 0;
 
@@ -362,17 +363,19 @@ struct AdamWList {
         c10::DeviceGuard guard(dev);
         const ppv_stream_t st = stream();
         std::vector<int64_t> now;
-        now.reserve(p.size() * 7 + 1);
+        now.reserve(p.size() * WORDS + 1);
         now.push_back(reinterpret_cast<int64_t>(st));
         for (size_t i = 0; i < p.size(); ++i) {
             const Tensor& g = p[i].grad();
             TORCH_CHECK_NOT_IMPLEMENTED(g.defined() && g.layout() == at::kStrided && g.scalar_type() == at::kFloat && g.is_contiguous() &&
-                                            g.device() == dev && is_plain(g) && is_plain(p[i]) && p[i].scalar_type() == at::kFloat && p[i].is_contiguous() && p[i].device() == dev &&
-                                            dev.is_cuda() && g.numel() == p[i].numel(),
+                                            g.device() == dev && is_plain(g) && is_plain(p[i]) && p[i].scalar_type() == at::kFloat &&
+                                            p[i].is_contiguous() && p[i].device() == dev && dev.is_cuda() && g.numel() == p[i].numel(),
                                         "ppv_amd.optim.AdamW: contiguous f32 parameters and gradients on one GPU only");
             const Tensor* held[] = {&p[i], &g, &m[i], &v[i], &ms[i], &vs[i]};
             for (const Tensor* t : held) now.push_back(t->defined() ? reinterpret_cast<int64_t>(t->data_ptr()) : 0);
             now.push_back(p[i].numel());
+            for (int k = 2; k < 6; ++k)                         // (another tensor, a shorter one, may lie where the old one lay)
+                now.push_back(held[k]->defined() ? held[k]->numel() * 128 + (int64_t)held[k]->scalar_type() * 2 + held[k]->is_contiguous() : 0);
         }
         if (now != key) {
             describe(now);
@@ -398,7 +401,7 @@ struct AdamWList {
         Tensor host = at::empty({(int64_t)(p.size() * sizeof(Record))}, at::TensorOptions().dtype(at::kByte).pinned_memory(true));
         auto* r = static_cast<Record*>(host.data_ptr());
         for (size_t i = 0; i < p.size(); ++i) {
-            const int64_t* at = now.data() + 1 + i * 7;
+            const int64_t* at = now.data() + 1 + i * WORDS;
             auto fits = [&](const Tensor& t, at::ScalarType kind, int64_t n) {
                 return t.scalar_type() == kind && t.numel() == n && t.is_contiguous() && t.device() == p[i].device();
             };

@@ -506,3 +506,26 @@ def test_a_refused_step_leaves_the_list_as_it_was(bits):
             o.step()
         runs.append([p.detach() for p in ps])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_a_state_that_became_shorter_or_another_type_in_its_place(bits):
+    """The same address does not make it the same tensor: a shorter one may lie where the old one lay."""
+    from ppv_amd.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(1024, device="cuda"))
+    p.grad = torch.ones(1024, device="cuda")
+    o = AdamW([p], state_bits=bits, min_8bit_size=256)
+    o.step()
+    for name, t in list(o.state[p].items()):
+        if not torch.is_tensor(t):
+            continue
+        keep = t.data
+        for other in (keep[:3], keep.view(torch.uint8)[:keep.numel()].view(torch.bool), keep.as_strided(keep.shape, (0,))):
+            t.data = other
+            assert t.data_ptr() == keep.data_ptr()
+            with pytest.raises(ValueError, match="does not belong"):
+                o.step()
+            t.data = keep
+    o.step()
+    assert o.state[p]["step"] == 2.0
