@@ -21,6 +21,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/version.h>
 
+#include <algorithm>
 #include <unordered_set>
 
 #include "ppv_hip.h"
@@ -339,6 +340,7 @@ struct AdamWList {
     std::vector<Tensor> p, m, v, ms, vs, rest;                 // rest: the group's parameters that had no gradient
     std::vector<int64_t> place, key;
     static constexpr int WORDS = 11;                           // of the key for each parameter: six addresses, its size, what its moments are
+    std::vector<std::pair<int64_t, int64_t>> spans;            // what a step writes, in order: addresses [from, to)
     Tensor table;
     int records = 0, blocks = 0;
 
@@ -418,11 +420,43 @@ struct AdamWList {
             x.place = (uint32_t)place[i];
             blk += (at[6] + 4095) / 4096;
         }
+        auto apart = spans_of(now);
         TORCH_CHECK(blk <= INT32_MAX, "ppv_amd.optim.AdamW: too many elements in one group");
         // pinned and non-blocking: a list whose gradients move every step does not wait for the device
         table = count ? host.to(p[0].device(), at::kByte, /*non_blocking=*/true) : Tensor();
         records = count;
         blocks = (int)blk;
+        spans = std::move(apart);
+    }
+
+    // The launch's workgroups write in any order: nothing they write may overlap, and no gradient may lie in it but a parameter's own (every
+    // element is read before it is written).
+    std::vector<std::pair<int64_t, int64_t>> spans_of(const std::vector<int64_t>& now) const {
+        bool moved = key.size() != now.size();
+        for (size_t i = 0; i < p.size() && !moved; ++i)
+            for (int k = 0; k < 7 && !moved; ++k) moved = k != 1 && key[1 + i * WORDS + k] != now[1 + i * WORDS + k];
+        std::vector<std::pair<int64_t, int64_t>> r = spans;
+        auto end = [&](int64_t from, const Tensor& t) { return from + (int64_t)t.nbytes(); };
+        if (moved) {
+            r.clear();
+            for (size_t i = 0; i < p.size(); ++i) {
+                const int64_t* at = now.data() + 1 + i * WORDS;
+                const Tensor* held[] = {&p[i], nullptr, &m[i], &v[i], &ms[i], &vs[i]};
+                for (int k = 0; k < 6; ++k)
+                    if (held[k] && held[k]->defined() && held[k]->numel()) r.emplace_back(at[k], end(at[k], *held[k]));
+            }
+            std::sort(r.begin(), r.end());
+            for (size_t i = 1; i < r.size(); ++i)
+                TORCH_CHECK_VALUE(r[i - 1].second <= r[i].first, "ppv_amd.optim.AdamW: parameters or moments of one group share memory");
+        }
+        for (size_t i = 0; i < p.size(); ++i) {
+            const int64_t* at = now.data() + 1 + i * WORDS;
+            if (at[6] == 0 || at[1] == at[0]) continue;
+            const auto next = std::upper_bound(r.begin(), r.end(), std::make_pair(at[1], INT64_MAX));
+            TORCH_CHECK_VALUE((next == r.end() || end(at[1], p[i]) <= next->first) && (next == r.begin() || std::prev(next)->second <= at[1]),
+                              "ppv_amd.optim.AdamW: a gradient and what the step writes share memory");
+        }
+        return r;
     }
 };
 

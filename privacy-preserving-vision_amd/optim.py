@@ -202,9 +202,6 @@ class AdamW(torch.optim.Optimizer):
             if not (all(t.device == p.device and t.is_contiguous() and t.numel() == n and t.dtype == kind for t in (m, v)) and (ms is None or all(
                     t.device == p.device and t.is_contiguous() and t.numel() == (n + 255) // 256 and t.dtype == torch.float32 for t in (ms, vs)))):
                 raise ValueError("ppv_amd.optim.AdamW: a parameter's state does not belong to it (type, size, device or layout)")
-        at = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in ps if p.numel())
-        if any(a[1] > b[0] for a, b in zip(at, at[1:])):
-            raise ValueError("ppv_amd.optim.AdamW: parameters of one group share memory")
         native = _lib.torch_ops().AdamWList(ps, held[0::4], held[1::4], held[2::4], held[3::4], [self._place[p] & 0xFFFFFFFF for p in ps])
         self._tables[slot] = (ps, held, native)
         return native

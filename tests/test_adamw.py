@@ -529,3 +529,52 @@ def test_adamw_refuses_a_state_that_became_shorter_or_another_type_in_its_place(
             t.data = keep
     o.step()
     assert o.state[p]["step"] == 2.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_refuses_memory_that_comes_to_be_shared(bits):
+    """Tensors of one launch that overlap would be written by two workgroups in any order: refused at the first step and at any later one that finds other
+    addresses, parameters, moments and scales alike; so is a gradient that lies in what the launch writes, but for a parameter's own."""
+    from ppv_amd.optim import AdamW
+    buf = torch.zeros(4096, device="cuda")
+    ps = [torch.nn.Parameter(torch.zeros(1024, device="cuda")) for _ in range(3)]
+    o = AdamW(ps, lr=1e-2, weight_decay=0.0, state_bits=bits, min_8bit_size=256)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    o.step()
+    names = [n for n, t in o.state[ps[0]].items() if torch.is_tensor(t)]
+    assert len(names) == (4 if bits == 8 else 2)
+
+    def refused(put, back):
+        put()
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share memory"):
+                o.step()
+        back()
+
+    keep = [p.data for p in ps]
+    def two(a, b):
+        ps[0].data, ps[2].data = a, b
+    def own():
+        for p, t in zip(ps, keep):
+            p.data = t
+    refused(lambda: two(buf[:1024], buf[1023:2047]), own)
+    refused(lambda: two(buf[1:1025], buf[:1024]), own)
+    for n in names:                                             # one moment for two parameters
+        st = o.state[ps[2]]
+        mine = st[n]
+        refused(lambda: st.__setitem__(n, o.state[ps[0]][n]), lambda: st.__setitem__(n, mine))
+    g = [p.grad for p in ps]
+    refused(lambda: setattr(ps[1], "grad", ps[0].data), lambda: setattr(ps[1], "grad", g[1]))
+    two(buf[:1024], keep[2])
+    refused(lambda: setattr(ps[0], "grad", buf[1:1025]), lambda: setattr(ps[0], "grad", g[0]))
+    own()
+    ps[1].grad = g[0]                                           # one gradient for two, neighbours, a gradient that is the parameter: in order
+    two(buf[:1024], buf[1024:2048])
+    o.step()
+    before = ps[0].detach().clone()
+    ps[0].grad = ps[0].data
+    o.step()
+    assert o.state[ps[0]]["step"] == 3.0 and torch.isfinite(ps[0]).all() and not torch.equal(ps[0], before)
+    assert torch.equal(buf[2048:], torch.zeros(2048, device="cuda"))
