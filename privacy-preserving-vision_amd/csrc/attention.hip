@@ -73,6 +73,11 @@ template <class T, int DP, int OG> struct FwdShape {
     static constexpr int WAVES = DP > 64 && sizeof(T) == 4 ? 1 : 2;         // per SIMD: 512 or 256 registers
 };
 
+// P enters the product with V in the operands' type, half a step of which is its error (bf16 2^-8, f16 2^-11, f32 none).  f16 also has a smallest number:
+// beside a largest P of 1 weights under 2^-25 would vanish, and a long history has enough of them to count (65536: 0.2 % of the result; l, in f32, would
+// hold them all the same).  There m stays 7 below the running maximum: P up to 2^7, 2^15 with the growth that is let pass, and weights down to 2^-32 count.
+template <class T> constexpr float P_LIFT = __is_same(T, f16s) ? 7.f : 0.f;
+
 template <class T, int DP, int OG>
 __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_kernel(const AttnFwd a) {
     using TL = Tile<T, DP>;
@@ -188,9 +193,9 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
             for (int j = 0; j < 16; ++j) top = fmaxf(top, s[mb][j]);
         top = half_swap_max(top) * c;
         // The running maximum follows only where it has grown by more than 2^8 (P, l and O then stay below 256 times what they would be: nothing
-        // to f32, and P's rounding is relative).  Without the hint the branch becomes 64 products and 64 copies in every tile.
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + 8.f) != 0, 0)) {
-            const float mn = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(mn == -__builtin_inff() ? 0.f : m - mn);
+        // to f32, and P's rounding is relative; 2^15 is in f16's range).  Without the hint the branch becomes 64 products and 64 copies in every tile.
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > m + (8.f + P_LIFT<T>)) != 0, 0)) {
+            const float mn = fmaxf(m, top - P_LIFT<T>), alpha = __builtin_amdgcn_exp2f(mn == -__builtin_inff() ? 0.f : m - mn);
             m = mn;
             l *= alpha;
 #pragma unroll

@@ -417,3 +417,25 @@ def test_attention_of_head_dimensions_between_64_and_96(B, Tq, Tk, H, Hkv, D, ca
     k_lens = torch.tensor([max(0, Tk - 5 * b) for b in range(B)], dtype=torch.int32)
     want, tol = _bounds(q, k, v, g, causal, None, k_lens, None)
     _check(NAMES, _run(q, k, v, g, causal=causal, k_lens=k_lens), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("B,Tq,Tk,H", [(8, 100, 4096, 32), (8, 40, 4096, 32), (64, 1, 8192, 8), (1, 1, 60000, 1)])
+def test_attention_of_one_large_score_among_many_small_ones(B, Tq, Tk, H, dt):
+    """One key whose weight is 2^25.2 times each other's, in a value of 0 among values of 1: what is left is the sum of the small weights, w = (Tk - 1)
+    e^-17.5.  As numbers of f16 beside a largest of 1 each of them would round to zero; beside one of 2^7 they are 2^-18.2, off by at most 2^-25, 2^-6.8 of
+    their value if all the same way.  bf16: half a step, 2^-8.  The values' sum is exact in f32 but for a chain of Tk / 32 additions."""
+    from ppv_amd.attention import multihead_attention
+    D, t = 16, DT[dt]
+    q, k, v = torch.zeros(B, Tq, H, D), torch.zeros(B, Tk, H, D), torch.ones(B, Tk, H, D)
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 1.0, 17.5, 0.0
+    q, k, v = (x.to(t).cuda() for x in (q, k, v))
+    w = (Tk - 1) * math.exp(-17.5)
+    want = w / (1.0 + w)
+    rel = {"f32": 0.0, "bf16": 2.0 ** -8, "f16": 2.0 ** -6.8}[dt] + torch.finfo(t).eps / 2 + (Tk / 32 + 64 + 16 * 17.5) * U
+    with torch.no_grad():
+        out = multihead_attention(q, k, v, scale=1.0)
+        first = multihead_attention(q, k.flip(1), v.flip(1), scale=1.0)          # the large one last
+    for o in (out, first):
+        assert ((o.double() - want).abs() <= want * rel + (2.0 ** -25 if dt == "f16" else 0.0)).all(), (float(o.min()), float(o.max()), want)
