@@ -5,6 +5,10 @@
 //
 // (The scale is in dS when it is rounded to the operands' type: its range in f16 is then that of the results.)
 //
+// dV's P is rounded to that type as well (half a step of it).  In f16 weights under 2^-25 would be zero there, and no scaled loss could help them: dK / dV
+// computes 2^12 P (one key of e^17.5 times the others' weight over 1500 rows: the others' dV 0 before, 3.75e-5 so), takes the 2^12 out of dP and D, which makes
+// dS what it is, and out of dV's sums at the end.
+//
 // Two launches, no atomics: the gradients have the same bits every time.
 //   attn_dq   a wave owns 32 rows (columns of S^T, dP^T, dQ^T) and walks over the keys; it also leaves D for the second launch
 //   attn_dkv  a wave owns 32 keys (columns of S, dP, dK^T, dV^T) and walks over the rows of all query heads that share them
@@ -259,6 +263,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     ST sq, so;
     float st = 0.f;
     int sl = -1;
+    constexpr float LIFT = __is_same(T, f16s) ? 12.f : 0.f, DOWN = __is_same(T, f16s) ? 0x1p-12f : 1.f;
     if (DIRECT && nch < TL::NCH) {
         clear_lds<DIRECT ? 4 * TL::bytes(QT) : NT * 16, NT>(smem, tid);
         __syncthreads();
@@ -277,6 +282,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         if (uwave < 2 * QT / 64) {
             const int r = rt * QT + tid % QT, rr = min(r, rows - 1), t = d.G == 1 ? rr : (int)((unsigned)rr / (unsigned)d.G);
             st = (tid < QT ? a.lse : a.delta)[((long)b * d.H + hk * d.G + (rr - t * d.G)) * d.Tq + t];
+            if constexpr (LIFT != 0.f) st = tid < QT ? st - LIFT : st * DOWN;
             sl = r >= rows ? -1 : d.causal ? min(klen - 1, t + shift) : klen - 1;
         }
     };
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         sv.fetch(V, key0, klen, nch, tid);
         sv.put(vown, tid);                                     // (the first tile's barrier comes before its first reader)
     } else load_own<T, DP>(vf, V, key, klen, nch, lane);
-    const float c = d.scale * LOG2E;
+    const float c = d.scale * LOG2E, scale = d.scale * DOWN;
     f32x16 dk[TL::DB], dv[TL::DB];
 #pragma unroll
     for (int i = 0; i < TL::DB; ++i)
@@ -334,7 +340,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
             for (int i = 0; i < 4; ++i) {
                 const int j = 4 * g + i;
                 const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], c, -lsv[i]));
-                s[j] = pe * __builtin_fmaf(p[j], d.scale, -dev[i]);
+                s[j] = pe * __builtin_fmaf(p[j], scale, -dev[i]);
                 p[j] = pe;
             }
         }
@@ -367,6 +373,11 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
     if (SG > 1) __syncthreads();
     if (!meet<TL::DB, OG, SG>(dv, (float*)smem, og, sg, lane) || !first_group) return;
     if (key >= d.Tk) return;
+    if constexpr (LIFT != 0.f)
+#pragma unroll
+        for (int i = 0; i < TL::DB; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) dv[i][j] *= DOWN;
     if (a.nsplit > 1) {
         float* pk = a.part + (((long)blockIdx.y * d.nbh + bh) * d.Tk + key) * DP;
         float* pv = pk + (long)a.nsplit * d.nbh * d.Tk * DP;

@@ -439,3 +439,21 @@ def test_attention_of_one_large_score_among_many_small_ones(B, Tq, Tk, H, dt):
         first = multihead_attention(q, k.flip(1), v.flip(1), scale=1.0)          # the large one last
     for o in (out, first):
         assert ((o.double() - want).abs() <= want * rel + (2.0 ** -25 if dt == "f16" else 0.0)).all(), (float(o.min()), float(o.max()), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Tq,Tk,H,Hkv", [(1500, 300, 2, 2), (700, 200, 16, 2), (64, 64, 32, 1), (3000, 20, 1, 1)])
+def test_attention_gradient_of_values_with_small_weights(Tq, Tk, H, Hkv, dt):
+    """Every row gives one key e^17.5 times each other's weight (2^-25.2); their dV is the sum of it over the rows, w = rows e^-17.5 / (1 + (Tk - 1) e^-17.5): a
+    scaled loss would not help numbers of f16 that round to zero beside 1; beside 2^12 they are 2^-13.2, no subnormal ones.  dQ and dK are 0: V is the same for all keys."""
+    D, t = 16, DT[dt]
+    q, k, v, g = torch.zeros(1, Tq, H, D), torch.zeros(1, Tk, Hkv, D), torch.ones(1, Tk, Hkv, D), torch.ones(1, Tq, H, D)
+    q[..., 0], k[:, 7, :, 0] = 1.0, 17.5
+    out, dq, dk, dv = _run(*(x.to(t) for x in (q, k, v, g)), scale=1.0)
+    rows = Tq * H // Hkv
+    w = rows * math.exp(-17.5) / (1.0 + (Tk - 1) * math.exp(-17.5))
+    h = torch.finfo(t).eps / 2
+    rel = h + (0.0 if dt == "f32" else h) + (rows / 32 + 64 + 16 * 17.5 + 32) * U
+    small = torch.cat([dv[:, :7], dv[:, 8:]], 1).double()
+    assert ((small - w).abs() <= w * rel + (2.0 ** -25 if dt == "f16" else 0.0)).all(), (float(small.min()), float(small.max()), w)
