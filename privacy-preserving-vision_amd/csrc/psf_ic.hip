@@ -867,7 +867,8 @@ __global__ __launch_bounds__(256) void psf_finalize_kernel(const float* __restri
     }
 }
 
-// backward of finalize: g_n = g_psf_m*m2 + g_psf_n + g_loss * psf_n*(m1-1)^2 / loss;  dots[l] += sum g_n * psf_n
+// backward of finalize: g_n = g_psf_m*m2 + g_psf_n + g_loss * psf_n*(m1-1)^2 / loss;  part[workgroup][l] = sum g_n * psf_n, which
+// psf_dots_kernel adds in a fixed order: with atomics the coefficient gradients of two equal calls differed in one of eight
 __global__ __launch_bounds__(256) void psf_finalize_bwd1_kernel(const float* __restrict__ psf_n,
                                                                 const double* __restrict__ m1,
                                                                 const double* __restrict__ m2,
@@ -875,7 +876,7 @@ __global__ __launch_bounds__(256) void psf_finalize_bwd1_kernel(const float* __r
                                                                 const float* __restrict__ g_psf_n,
                                                                 const double* __restrict__ g_loss,
                                                                 const double* __restrict__ loss, double* __restrict__ g_n,
-                                                                double* __restrict__ dots, long n) {
+                                                                double* __restrict__ part, long n) {
     __shared__ double s_red[4][3];
     const long idx = (long)blockIdx.x * 256 + threadIdx.x;
     double acc[3] = {0, 0, 0};
@@ -903,7 +904,27 @@ __global__ __launch_bounds__(256) void psf_finalize_bwd1_kernel(const float* __r
     __syncthreads();
     if (threadIdx.x < 3) {
         const int l = threadIdx.x;
-        atomicAdd(&dots[l], s_red[0][l] + s_red[1][l] + s_red[2][l] + s_red[3][l]);
+        part[(long)blockIdx.x * 3 + l] = s_red[0][l] + s_red[1][l] + s_red[2][l] + s_red[3][l];
+    }
+}
+// dots[l] = sum over n workgroups of part[.][l]
+__global__ __launch_bounds__(256) void psf_dots_kernel(const double* __restrict__ part, double* __restrict__ dots, long n) {
+    __shared__ double s_red[4][3];
+    double acc[3] = {0, 0, 0};
+    for (long i = threadIdx.x; i < n; i += 256)
+#pragma unroll
+        for (int l = 0; l < 3; ++l) acc[l] += part[i * 3 + l];
+#pragma unroll
+    for (int l = 0; l < 3; ++l) {
+        double a = acc[l];
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) a += __shfl_xor(a, off, 64);
+        if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6][l] = a;
+    }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        const int l = threadIdx.x;
+        dots[l] = s_red[0][l] + s_red[1][l] + s_red[2][l] + s_red[3][l];
     }
 }
 
@@ -970,7 +991,7 @@ struct IcWs {            // carve-up of the caller's persistent state buffer (sa
     float* raw;          // [P][P][3]
     double* sums;        // [3] + dots[3] + loss_acc[1] + pad
     double* g_n;         // [P*P*3]
-    double* part;        // [nwg][K]
+    double* part;        // [nwg][K]; before that [workgroups of P * P * 3][3]
     float* gh;           // [RR*RR]
     unsigned char* support;   // [RR*RR/4] basis support per float4 group (ppv_ic_psf_mark_support), behind a one-byte "marked" flag
     unsigned char* sym;       // mirror symmetry of the basis: 256-byte header (SymHdr), [K] u32 sign-pair sets, [K] u8 classes
@@ -993,7 +1014,8 @@ size_t carve(IcWs* w, char* base, int RR, int P, int K) {
     w->sums = (double*)take(8 * 8);
     w->g_n = (double*)take((size_t)P * P * 3 * 8);
     const size_t nwg = (npx / 4 + 255) / 256;
-    w->part = (double*)take(nwg * 4 * K * 8);
+    const size_t ndot = ((size_t)P * P * 3 + 255) / 256;       // (psf_finalize_bwd1_kernel's sums: used up before the basis pass writes there)
+    w->part = (double*)take((nwg * 4 * K > ndot * 3 ? nwg * 4 * K : ndot * 3) * 8);
     w->gh = (float*)take(npx * 4);
     w->support = (unsigned char*)take(npx / 4 + 256);          // 256-byte header (magic word) + one byte per float4 group
     w->sym = (unsigned char*)take(256 + (size_t)K * 5);
@@ -1122,9 +1144,9 @@ int psf_bwd_t(const float* Z, const void* Ht, const double* kdn, const double* m
     C2 *F0 = (C2*)w.F0, *U = (C2*)w.U, *T1 = (C2*)w.T1, *T2 = (C2*)w.T2;
     const long npx = (long)RR * RR, n = (long)P * P * 3;
     double* dots = w.sums + 3;
-    (void)hipMemsetAsync(dots, 0, 24, stream);
     psf_finalize_bwd1_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(psf_n, m1, m2, g_psf_m, g_psf_n, g_loss, loss,
-                                                                            w.g_n, dots, n);
+                                                                            w.g_n, w.part, n);
+    psf_dots_kernel<<<1, 256, 0, stream>>>(w.part, dots, (n + 255) / 256);
     C2* GU = T2;      // T2 is dead after forward and holds 3*RR*M >= 3*RR*RR elements; U and F0 stay intact
     area_down_bwd_kernel<C2><<<(unsigned)((npx + 255) / 256), 256, 0, stream>>>(w.g_n, dots, w.sums, U, GU, RR, P, up, up_scale);
     if (dfft_static(M)) dfft_rows_kernel<true, C2><<<3 * RR, 256, 0, stream>>>(GU, T1, tw, pl, RR, pad);
