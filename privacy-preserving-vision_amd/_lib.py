@@ -263,7 +263,8 @@ _TORCH_ENTRIES = ("ppv_layernorm_fwd", "ppv_layernorm_bwd", "ppv_layernorm_bwd_w
 def _check_torch_ops(mod):
     """A ppv_torch.so that was compiled against another header or torch would hand over structures of another layout."""
     built = (getattr(mod, "abi_version", None), getattr(mod, "attention_bytes", None), getattr(mod, "torch_version", None))
-    if built != (ABI_VERSION, ctypes.sizeof(Attention), torch.__version__.split("+")[0]):
+    release = re.match(r"\d+\.\d+\.\d+", torch.__version__)                   # (the header has no more of it: "2.10.0a0+git" is "2.10.0" there)
+    if built != (ABI_VERSION, ctypes.sizeof(Attention), release and release.group()):
         raise RuntimeError(f"{TORCH_LIB_PATH}: compiled for ABI version {built[0]} (PpvAttention of {built[1]} bytes) and torch {built[2]}, loaded with "
                            f"ABI version {ABI_VERSION} ({ctypes.sizeof(Attention)} bytes) and torch {torch.__version__} (stale build? re-run __graft_entry__.build())")
 

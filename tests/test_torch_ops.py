@@ -139,3 +139,14 @@ def test_a_library_of_another_build_is_refused():
             _lib._check_torch_ops(types.SimpleNamespace(**{**{n: getattr(mod, n) for n in names}, name: other}))
     with pytest.raises(RuntimeError, match="stale build"):
         _lib._check_torch_ops(types.SimpleNamespace())          # from before it said what it was made for
+
+
+@pytest.mark.parametrize("version", ["", "a0+git1234567", ".dev20260101+rocm7.0", "+rocm7.0"])
+def test_builds_of_one_torch_release_are_one(version, monkeypatch):
+    from ppv_amd import _lib
+    mod = _lib.torch_ops()
+    monkeypatch.setattr(torch, "__version__", mod.torch_version + version)
+    _lib._check_torch_ops(mod)
+    monkeypatch.setattr(torch, "__version__", mod.torch_version + "7" + version)
+    with pytest.raises(RuntimeError, match="stale build"):
+        _lib._check_torch_ops(mod)
