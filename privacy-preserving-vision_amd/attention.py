@@ -60,8 +60,9 @@ def multihead_attention(q, k, v, causal=False, q_lens=None, k_lens=None, scale=N
     q_lens, k_lens  int32 / int64 [B] on the same device (clamped to 0..Tq, 0..Tk): a sequence's queries and keys at or behind its length take
                     no part, whatever they hold; such queries give zeros, such queries and keys zero gradients.
     causal          row i of a sequence with n queries and m keys sees key j if j <= i + m - n: the last query sees every key, so a single new token
-                    sees its whole history.  Rows that see nothing give zeros and zero gradients.  (An infinite or NaN
-                    value in a key or row can reach, as zero times infinity, rows and keys of its sequence that do not see it.)
+                    sees its whole history.  Rows that see nothing, or whose scores are all minus infinity, give zeros and zero
+                    gradients.  (An infinite or NaN value in a key or row can reach, as zero times infinity, rows and keys of its
+                    sequence that do not see it.)
     scale           > 0, D ** -0.5 by default.
 
     Fewer than 2^30 rows of a sequence (times heads), keys, and (sequence, key head) pairs; 2^24 tiles of 32 to 128 rows or keys in all.

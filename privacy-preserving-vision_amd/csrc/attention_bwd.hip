@@ -3,6 +3,7 @@
 //     P = exp2(scale log2e Q K^T - lse),   dP = dO V^T,   D = scale rowsum(dO O),   dS = P (scale dP - D)
 //     dQ = dS K,   dK = dS^T Q,   dV = P^T dO
 //
+// (A row with lse = -inf has no key, or scores of -inf alone: read as +inf it makes P zero in either case, as the forward pass has it.)
 // (The scale is in dS when it is rounded to the operands' type: its range in f16 is then that of the results.)
 //
 // dV's P is rounded to that type as well (half a step of it).  In f16 weights under 2^-25 would be zero there, and no scaled loss could help them: dK / dV
@@ -31,6 +32,8 @@ struct AttnBwd {
     float* part;                                               // nsplit > 1: f32 sums [nsplit][nbh][rows or Tk][DP] (dK, then dV)
     int ntile, nsplit;
 };
+
+__device__ __forceinline__ float lse_or_none(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse; }
 
 // a split's share [t0, t1) of the tiles that a workgroup walks over
 __device__ __forceinline__ void attn_share(int nsplit, int& t0, int& t1) {
@@ -145,7 +148,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 1>::WAVES)) void attn_dq_
     const long stat = ((long)b * d.H + h) * d.Tq + tok;
     float lse = 0.f;
     if (row < rows) {
-        lse = a.lse[stat];
+        lse = lse_or_none(a.lse[stat]);
         if (half == 0 && sg == 0 && blockIdx.y == 0) a.delta[stat] = delta;
     }
     const float c = d.scale * LOG2E;
@@ -282,6 +285,7 @@ __global__ __launch_bounds__(256, (BwdShape<T, DP, OG, 2>::WAVES)) void attn_dkv
         if (uwave < 2 * QT / 64) {
             const int r = rt * QT + tid % QT, rr = min(r, rows - 1), t = d.G == 1 ? rr : (int)((unsigned)rr / (unsigned)d.G);
             st = (tid < QT ? a.lse : a.delta)[((long)b * d.H + hk * d.G + (rr - t * d.G)) * d.Tq + t];
+            if (tid < QT) st = lse_or_none(st);
             if constexpr (LIFT != 0.f) st = tid < QT ? st - LIFT : st * DOWN;
             sl = r >= rows ? -1 : d.causal ? min(klen - 1, t + shift) : klen - 1;
         }

@@ -457,3 +457,28 @@ def test_attention_gradient_of_values_with_small_weights(Tq, Tk, H, Hkv, dt):
     rel = h + (0.0 if dt == "f32" else h) + (rows / 32 + 64 + 16 * 17.5 + 32) * U
     small = torch.cat([dv[:, :7], dv[:, 8:]], 1).double()
     assert ((small - w).abs() <= w * rel + (2.0 ** -25 if dt == "f16" else 0.0)).all(), (float(small.min()), float(small.max()), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("Tq,Tk,H,Hkv", [(40, 33, 2, 2), (200, 300, 4, 2), (1, 3000, 1, 1)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_rows_whose_scores_all_overflow(Tq, Tk, H, Hkv, causal, dt):
+    """A row that gives every key it sees a score of minus infinity (products of 1e25 and -1e25) is like one that sees nothing: zeros, and it takes no part in the
+    gradients.  The other rows and the keys are as without it."""
+    D = 32
+    q, k, v, g = _inputs(1, Tq, Tk, H, Hkv, D, DT[dt], Tq + Tk)
+    row = Tq // 2
+    q[..., 0], k[..., 0] = 0.0, -1e25
+    q[0, row, :, 0] = 1e25
+    out, dq, dk, dv = _run(q, k, v, g, causal=causal)
+    for t in (out[0, row], dq[0, row]):
+        assert torch.equal(t, torch.zeros_like(t))
+    assert all(torch.isfinite(t).all() for t in (out, dq, dk, dv))
+    k2, g2, q2 = k.clone(), g.clone(), q.clone()
+    k2[..., 0], g2[0, row], q2[0, row] = 0.0, 0.0, 0.0
+    want, tol = _bounds(q2, k2, v, g2, causal, None, None, None)
+    keep = [i for i in range(Tq) if i != row]
+    # (dq of the row's first dimension is a sum of dS times -1e25: not finite in general, left out for the others, as is dk's, a sum of dS times 0 or 1e25)
+    _check(("out", "dq", "dk", "dv"), (out[:, keep], dq[:, keep, :, 1:], dk[..., 1:], dv),
+           (want[0][:, keep], want[1][:, keep, :, 1:], want[2][..., 1:], want[3]), (tol[0][:, keep], tol[1][:, keep, :, 1:], tol[2][..., 1:], tol[3]))
