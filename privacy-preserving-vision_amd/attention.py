@@ -6,8 +6,9 @@ with caption tokens and with the encoder's cells or pixels, next to the single-s
 
 Scores and probabilities are never stored: the forward pass keeps one number per row (the log of the softmax's denominator), the backward
 pass computes the probabilities again from it.  Products run on the matrix pipe in the operands' type (f32: exact f32 products) and
-accumulate in f32; softmax statistics are f32, the probabilities are rounded to the operands' type where they enter the next product.  No atomics: the
-same bits every time.  No CPU path."""
+accumulate in f32; softmax statistics are f32.  Where probabilities and their gradients enter the next product they are rounded to the operands' type, or,
+where that costs nothing (up to 32 rows or keys to a key head), given in two terms of it (csrc/attention_tiles.h two_terms).  No atomics: the same
+bits every time.  No CPU path."""
 import torch
 
 from . import _lib

@@ -73,7 +73,7 @@ template <class T, int DP, int OG> struct FwdShape {
     static constexpr int WAVES = DP > 64 && sizeof(T) == 4 ? 1 : 2;         // per SIMD: 512 or 256 registers
 };
 
-// P enters the product with V in the operands' type, half a step of which is its error (bf16 2^-8, f16 2^-11, f32 none).  f16 also has a smallest number:
+// P enters the product with V in the operands' type, in one term or two (attention_tiles.h two_terms).  f16 also has a smallest number:
 // beside a largest P of 1 weights under 2^-25 would vanish, and a long history has enough of them to count (65536: 0.2 % of the result; l, in f32, would
 // hold them all the same).  There m stays 7 below the running maximum: P up to 2^7, 2^15 with the growth that is let pass, and weights down to 2^-32 count.
 template <class T> constexpr float P_LIFT = __is_same(T, f16s) ? 7.f : 0.f;
@@ -219,8 +219,14 @@ __global__ __launch_bounds__(256, (FwdShape<T, DP, OG>::WAVES)) void attn_fwd_ke
 #pragma unroll
             for (int kf = 0; kf < TL::CF; ++kf) {
                 const u32x4 pf = TL::from_acc(s[mb], kf);
+                u32x4 pr;
+                if constexpr (two_terms<T, OG>) pr = TL::rest_of_acc(s[mb], kf, pf);
 #pragma unroll
-                for (int i = 0; i < TL::DB; ++i) o[i] = TL::mma(TL::by_col(tv, L, own + mb * 32, i, kf), pf, o[i]);
+                for (int i = 0; i < TL::DB; ++i) {
+                    const u32x4 vt = TL::by_col(tv, L, own + mb * 32, i, kf);
+                    o[i] = TL::mma(vt, pf, o[i]);
+                    if constexpr (two_terms<T, OG>) o[i] = TL::mma(vt, pr, o[i]);
+                }
             }
         __builtin_amdgcn_s_setprio(0);
     }

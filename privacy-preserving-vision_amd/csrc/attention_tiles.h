@@ -93,6 +93,15 @@ template <class T, int DP> struct Tile {
             return v;
         }
     }
+    // what rounding took from from_acc's result, as another fragment of the type
+    static __device__ __forceinline__ u32x4 rest_of_acc(const f32x16& c, int kf, u32x4 hi) {
+        static_assert(ES == 2, "f32 fragments are the registers themselves");
+        float v[8];
+        unpack_vec<T>(hi, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c[8 * kf + e] - v[e];
+        return pack_vec<T>(v);
+    }
     static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
         if constexpr (__is_same(T, bf16s))
             return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_, a), __builtin_bit_cast(bf16x8_, b), c, 0, 0, 0);
@@ -106,6 +115,14 @@ template <class T, int DP> struct Tile {
         }
     }
 };
+
+// P and dS enter the next product in the operands' 16-bit type.  One term of it is off by half a step (bf16 2^-8, f16 2^-11), which adds to the half step of
+// the results' own rounding: 1.35 to 1.45 times the error of a computation in 32 bits that is rounded once.  Two terms (the rounded value and
+// what that took) leave the results' rounding alone and cost one more product each.  They are taken where products are not what takes the time: one wave
+// owns all rows (keys) of its problem, up to 32, and the walk is bound by the bytes of K and V (Q and dO).  One token of 32 heads on 8, 4 x 65536 keys of
+// 128, bf16: 205 us either way; 128 x 32 rows on 1296 keys, 8 heads of 64, both directions: 379 either way.  Where many rows keep the matrix
+// pipe busy they would cost a quarter (2 x 16 heads of 4096, D = 32, causal: forward 79 -> 99 us, both directions 297 -> 379).
+template <class T, int OG> constexpr bool two_terms = sizeof(T) == 2 && OG == 1;
 
 // The problem, as the kernels take it (elements, not bytes).  Token strides, head strides and batch strides are multiples of 16 bytes.
 struct AttnDims {

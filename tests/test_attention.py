@@ -482,3 +482,31 @@ def test_attention_rows_whose_scores_all_overflow(Tq, Tk, H, Hkv, causal, dt):
     # (dq of the row's first dimension is a sum of dS times -1e25: not finite in general, left out for the others, as is dk's, a sum of dS times 0 or 1e25)
     _check(("out", "dq", "dk", "dv"), (out[:, keep], dq[:, keep, :, 1:], dk[..., 1:], dv),
            (want[0][:, keep], want[1][:, keep, :, 1:], want[2][..., 1:], want[3]), (tol[0][:, keep], tol[1][:, keep, :, 1:], tol[2][..., 1:], tol[3]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hkv,D", [(2, 1, 700, 4, 2, 64), (3, 5, 300, 8, 2, 128), (1, 32, 2000, 2, 2, 96), (2, 9, 9, 4, 1, 80), (2, 100, 30, 2, 2, 64), (1, 300, 300, 2, 1, 8),
+                                             (2, 70, 200, 3, 3, 32), (1, 4, 5000, 1, 1, 40)])
+def test_attention_of_few_rows_or_keys_rounds_its_results_alone(B, Tq, Tk, H, Hkv, D, dt):
+    """Where the matrix products are not what takes the time (up to 32 rows to a key head: value and dQ; up to 32 keys: dK and dV; D up to 32: dQ) P and dS enter them in two
+    terms of the 16-bit type, off by h^2 of their value (f16 also by half a step of its subnormals, 2^-25, beside a P of at least 2^7 in the value's product,
+    2^12 P in dV's and dS itself in dQ's and dK's).  The rest is that of f32 operands, and the result's one rounding."""
+    t = DT[dt]
+    q, k, v, g = _inputs(B, Tq, Tk, H, Hkv, D, t, Tq + 7 * Tk + D)
+    want, tol = _bounds(q.float(), k.float(), v.float(), g.float(), False, None, None, None)
+    h, tiny, G, scale = torch.finfo(t).eps / 2, 2.0 ** -25 if dt == "f16" else 0.0, H // Hkv, D ** -0.5
+    qh, gh = (x.double().transpose(1, 2) for x in (q, g))                                          # [B, H, Tq, D]
+    kh, vh = (x.double().transpose(1, 2).repeat_interleave(G, 1) for x in (k, v))
+    p = torch.softmax(qh @ kh.transpose(2, 3) * scale, -1)
+    ds = (p * (gh @ vh.transpose(2, 3) - (gh * (p @ vh)).sum(-1, keepdim=True)) * scale).abs()
+    heads = lambda x: x.view(B, Hkv, G, Tk, D).sum(2)
+    few, keys = Tq * G <= 32, Tk <= 32
+    # D = rowsum(dO O) is the forward pass' O, whose P has one term where there are more rows: off by h sum |dO| sum P |V|, and dS by P times that
+    d_off = 0.0 if few else h * scale * p * (gh.abs() * (p @ vh.abs())).sum(-1, keepdim=True)
+    two = [(h * h * p + 2.0 ** -7 * tiny) @ vh.abs(), (h * h * ds + d_off + tiny) @ kh.abs(), heads((h * h * ds + d_off + tiny).transpose(2, 3) @ qh.abs()),
+           heads((h * h * p + 2.0 ** -12 * tiny).transpose(2, 3) @ gh.abs())]
+    got = _run(q, k, v, g)
+    for name, a, b, s, x, on in zip(NAMES, got, want, tol, two, (few, few or D <= 32, keys, keys)):
+        if on:
+            _check((name,), (a,), (b,), (s + x.transpose(1, 2) + h * b.abs() + tiny,))
