@@ -9,12 +9,13 @@
 //     key tile staged in LDS is shared by the row groups and divided among the key groups, whose (O, m, l) meet in LDS at the end;
 //   * the next tile is on its way during the products: straight into the other LDS buffer (16-bit types), else into registers;
 //   * rows behind a sequence's end and rows that see no key are zeros, with -inf; keys behind the end are not read;
-//   * few rows: the keys are split over workgroups in units of equal length whatever the sequences' lengths, each leaves (O, m, l) in f32,
-//     a second launch joins them.
-// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: 155 us = 885 TFLOP/s (a large library product: 1242); the matrix pipe is busy
-// 39 % of the cycles, the vector ALU 40 %, and they hardly overlap (the next tile's scores made while this one's softmax runs: 163 us and more); one token of 32 heads on
-// 8 key heads of 128 against 4 ragged histories of up to 65536: 772 MB in 140-150 us = 5.5-5.1 TB/s, and 6 us for the join; 32 x 52 rows against 1296
-// f32 keys, 8 heads of 64: 61 us, the f32 matrix pipe busy 60 % of them.
+//   * few rows and up to 170 tiles of them: the keys are split over workgroups in units of equal length whatever the sequences' lengths, each leaves
+//     (O, m, l) in f32, a second launch joins them.
+// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: 155 us = 885 TFLOP/s (a large library product: 1242); of the cycles in
+// which the CUs are busy the matrix pipe works in 45 %, the vector ALU in 45 %, and they hardly overlap (the next tile's scores made while this one's
+// softmax runs: 163 us and more); one token of 32 heads on
+// 8 key heads of 128 against 4 ragged histories of up to 65536: 772 MB in 140-155 us = 5.5-5.0 TB/s, and 6 us for the join; 32 x 52 rows against 1296
+// f32 keys, 8 heads of 64: 62 us, the f32 matrix pipe at work in 60 % of them.
 #include "attention_tiles.h"
 
 namespace ppv {
@@ -377,7 +378,9 @@ static AttnPlan attn_fwd_plan(int B, int Hkv, int G, int Tq, int Tk, int D, int 
     p.dp = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128;
     p.og = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
     p.ntile = (int)((rows + p.og * 32 - 1) / (p.og * 32));
-    // split where the tiles alone leave the chip idle: at most 512 workgroups (two for each CU, all of them resident: with 544 the last
+    // split where the tiles alone are fewer than a third of what is resident (one token, 8 key heads of 128, bf16, B sequences of 16384 keys: 168 tiles,
+    // split, 4.55 TB/s; 176 to 512, each a walk over its whole sequence, 4.7 to 5.8.  With lengths from a quarter to the whole 4.5 split, but 3.2 for 176, 4.3
+    // for 256 and 5.0 for 512 tiles, where the longest walk ends alone): at most 512 workgroups (two for each CU, all of them resident: with 544 the last
     // 32 of a history of 65536 keys ran alone, 179 us instead of 149), with at least two key tiles each
     const long base = (long)B * Hkv * p.ntile, kt = p.og == 4 ? (es == 2 ? 64 : 32) : p.og == 2 ? 64 : 128, ktiles = (Tk + kt - 1) / kt;
     long s = base >= 256 ? 1 : 512 / base - 1;

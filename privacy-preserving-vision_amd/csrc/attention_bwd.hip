@@ -6,9 +6,9 @@
 // (A row with lse = -inf has no key, or scores of -inf alone: read as +inf it makes P zero in either case, as the forward pass has it.)
 // (The scale is in dS when it is rounded to the operands' type: its range in f16 is then that of the results.)
 //
-// dV's P is rounded to that type as well (in one term or two: attention_tiles.h two_terms).  In f16 weights under 2^-25 would be zero there, and no scaled loss could help them: dK / dV
-// computes 2^12 P (one key of e^17.5 times the others' weight over 1500 rows: the others' dV 0 before, 3.75e-5 so), takes the 2^12 out of dP and D, which makes
-// dS what it is, and out of dV's sums at the end.
+// dV's P is rounded to that type as well (in one term or two: attention_tiles.h two_terms).  In f16 weights under 2^-25 would be zero there, and no
+// scaled loss could help them: dK / dV computes 2^12 P (one key of e^17.5 times the others' weight over 1500 rows: the others' dV 3.75e-5, else 0),
+// takes the 2^12 out of dP and D, which makes dS what it is, and out of dV's sums at the end.
 //
 // Two launches, no atomics: the gradients have the same bits every time.
 //   attn_dq   a wave owns 32 rows (columns of S^T, dP^T, dQ^T) and walks over the keys; it also leaves D for the second launch
@@ -16,8 +16,8 @@
 // That is 7 products where one launch with atomics on dQ would need 5.  Where few rows (keys) leave the chip idle, the axis that is walked over is
 // split; the splits' f32 sums are added in their order by a small launch.  Bound by the matrix pipe and, behind it, the LDS: every operand of a
 // tile is read along its rows (S, dP) and across them (dQ, dK, dV).
-// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: dQ 215 us = 960 TFLOP/s, dK / dV 290 us = 945; f32, 32 x 52 rows against
-// 1296 keys, 8 heads of 64: 80 and 137 us, the f32 matrix pipe busy 71 and 61 %.
+// Measured (MI355X): 2 x 16 heads of 4096 tokens, D = 128, bf16, causal: dQ 214 us = 960 TFLOP/s, dK / dV 295 us = 930; f32, 32 x 52 rows against
+// 1296 keys, 8 heads of 64: 82 and 141 us, the f32 matrix pipe at work in 69 and 59 % of the CUs' busy cycles.
 #include "attention_tiles.h"
 
 namespace ppv {

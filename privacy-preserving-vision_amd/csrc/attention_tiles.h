@@ -121,7 +121,8 @@ template <class T, int DP> struct Tile {
 // what that took) leave the results' rounding alone and cost one more product each.  They are taken where products are not what takes the time: one wave
 // owns all rows (keys) of its problem, up to 32, and the walk is bound by the bytes of K and V (Q and dO).  One token of 32 heads on 8, 4 x 65536 keys of
 // 128, bf16: 205 us either way; 128 x 32 rows on 1296 keys, 8 heads of 64, both directions: 379 either way.  Where many rows keep the matrix
-// pipe busy they would cost a quarter (2 x 16 heads of 4096, D = 32, causal: forward 79 -> 99 us, both directions 297 -> 379).
+// pipe busy they would cost a quarter (2 x 16 heads of 4096, D = 32, causal: forward 79 -> 99 us, both directions 297 -> 379).  The dearest
+// of what takes them, one token of 88 x 2 heads of 32 on 22456 f16 keys, went from 202 to 213 us.
 template <class T, int OG> constexpr bool two_terms = sizeof(T) == 2 && OG == 1;
 
 // The problem, as the kernels take it (elements, not bytes).  Token strides, head strides and batch strides are multiples of 16 bytes.

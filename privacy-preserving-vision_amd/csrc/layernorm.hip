@@ -10,9 +10,9 @@
 // Both directions: a fixed grid strides over the rows, the parameters are in registers, the next row is on its way while one is worked on.
 // Backward: every lane keeps the weight-gradient sums of its columns in registers, a workgroup leaves one partial row, a second launch adds the partial rows in their order (no atomics:
 // the same bits every time).
-// Measured (MI355X, bytes read and written once): 165888 x 2048 bf16 forward 5.4 TB/s, backward 5.5 (620 us together; 560 for backward alone without
-// the next row's loads); f32 5.0-5.7 and 4.9-5.6 at any C; 16-bit rows of an odd C, which start off every dword, 4 and 2.6-4.4; rows longer than
-// 8192, read again for each pass, 2.4-3.4 and 1.6-2.5.  6656 x 512 bf16: 5 + 8 + 4 us, less than the host takes to ask for them.
+// Measured (MI355X, bytes read and written once): 165888 x 2048 bf16 forward 266 us = 5.1 TB/s, backward 369 + 4 = 5.5 (638 us a pass; 816 without the next
+// row's loads in the backward kernel); f32 of 300 columns and more 4.7-5.7 and 4.9-5.5; 16-bit rows of an odd C, which start off every dword, 3.9-4.6 and
+// 2.6-4.3; rows longer than 8192, read again for each pass, 2.4-3.4 and 1.6-2.5.  6656 x 512 bf16: 6 + 8 + 4 us, less than the host takes to ask for them.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include "ppv_common.h"

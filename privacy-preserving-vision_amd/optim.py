@@ -117,8 +117,9 @@ class AdamW(torch.optim.Optimizer):
     place in the optimiser and the element's place in the tensor: the same run gives the same bits.
 
     Parameters and gradients are contiguous f32 tensors of one GPU per group; parameters without a gradient are left alone and keep their own
-    step count (a float).  Refused: amsgrad, maximize, capturable, sparse gradients, and a step inside a stream capture (the step's number is part of
-    the launch, a replay would repeat it)."""
+    step count (a float).  A step raises the versions of the parameters and moments that it wrote.  Refused: amsgrad, maximize, capturable, sparse
+    gradients, tensors of one group that share memory (but for a parameter that is its own gradient), and a step inside a stream capture (the
+    step's number is part of the launch, a replay would repeat it)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False, *, maximize=False, capturable=False,
                  state_bits=32, min_8bit_size=4096, seed=0):
