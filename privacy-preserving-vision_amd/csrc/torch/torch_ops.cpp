@@ -72,6 +72,15 @@ constexpr c10::DispatchKeySet stand_ins({c10::DispatchKey::Python, c10::Dispatch
 bool is_plain(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
 Tensor plain(const Tensor& t) { return is_plain(t) ? t : t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
 
+// A saved tensor as the backward pass finds it: saved-tensor hooks may have moved it away and back (other strides are read as they are), but what
+// the kernels read by address has to be of this size, type and device.
+Tensor saved_as(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == sizes && t.scalar_type() == type && t.device() == device &&
+                    !t.key_set().has_any(stand_ins),
+                "ppv_amd: a saved tensor came back from its hooks with another size, type or device");
+    return plain(t);
+}
+
 // The kernels go by addresses, out of sight of torch's dispatcher.  What it does besides computing would be missing from the result without a word;
 // the arguments of both operators, and the gradients that come back to them, are looked over for it: forward-mode tangents, and whoever records the
 // dispatched calls to run them again (torch.jit.trace, make_fx) or to run them without data: the record would be the allocation of the result alone;
@@ -170,12 +179,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             refuse_unseen("layer_norm", {&grads[0]});
             refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
-            const Tensor &x2 = saved[0], &w = saved[1], &stats = saved[2], &g = grads[0];
-            c10::DeviceGuard guard(x2.device());
-            const int64_t rows = x2.size(0), C = x2.size(1);
-            const Tensor g2 = rows_of(g, C);
+            const Tensor& g = grads[0];
+            c10::DeviceGuard guard(g.device());
+            const int64_t C = g.size(-1), rows = g.numel() / C;
             const auto par = (at::ScalarType)ctx->saved_data["par"].toInt();
             const int64_t has = ctx->saved_data["has"].toInt();                             // (a node's edges are those of the tensors it was given)
+            const Tensor g2 = rows_of(g, C), x2 = rows_of(saved_as(saved[0], {rows, C}, g.scalar_type(), g.device()), C);
+            const Tensor w = has & 1 ? saved_as(saved[1], {C}, par, g.device()).contiguous() : Tensor();
+            const Tensor stats = saved_as(saved[2], {2, rows}, at::kFloat, g.device()).contiguous();
             const bool want_w = (has & 1) && ctx->needs_input_grad(1), want_b = (has & 2) && ctx->needs_input_grad(1 + (has & 1));
             Tensor dx = at::empty({rows, C}, x2.options()), dw, db, ws;
             if (want_w) dw = at::empty({C}, x2.options().dtype(par));
@@ -228,6 +239,10 @@ Tensor operand(const Tensor& t, int64_t Dp) {
     if (Dp != t.size(3)) p.narrow(3, t.size(3), Dp - t.size(3)).zero_();
     p.narrow(3, 0, t.size(3)).copy_(t);
     return p;
+}
+// ... and as they write it: without gaps, from a multiple of 16 bytes
+Tensor packed(const Tensor& t) {
+    return t.is_contiguous() && reinterpret_cast<size_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 long stride_of(const Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
@@ -288,7 +303,6 @@ struct Attention : torch::autograd::Function<Attention> {
         ctx->save_for_backward({f.q, f.k, f.v, f.out, f.lo, f.lse, ql, kl});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
-        ctx->saved_data["D"] = q.size(3);
         return unpadded(f.out, q.size(3));
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -298,16 +312,26 @@ struct Attention : torch::autograd::Function<Attention> {
             refuse_unseen("multihead_attention", {&grads[0]});
             refuse_capture_of_eager_graph();
             const auto saved = ctx->get_saved_variables();
-            const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3];
-            c10::DeviceGuard guard(q.device());
-            const int64_t D = ctx->saved_data["D"].toInt();
+            const Tensor& go = grads[0];
+            c10::DeviceGuard guard(go.device());
+            const auto type = go.scalar_type();
+            const auto on = go.device();
+            const int64_t B = go.size(0), Tq = go.size(1), H = go.size(2), D = go.size(3), w = 16 / go.element_size(), Dp = (D + w - 1) / w * w;
+            const Tensor q = operand(saved_as(saved[0], {B, Tq, H, Dp}, type, on), Dp);
+            TORCH_CHECK(saved[1].dim() == 4, "ppv_amd: a saved tensor came back from its hooks with another size, type or device");
+            const int64_t Tk = saved[1].size(1), Hkv = saved[1].size(2);
+            const Tensor k = operand(saved_as(saved[1], {B, Tk, Hkv, Dp}, type, on), Dp), v = operand(saved_as(saved[2], {B, Tk, Hkv, Dp}, type, on), Dp);
+            TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "ppv_amd: a saved tensor came back from its hooks with another size, type or device");
+            const Tensor out = packed(saved_as(saved[3], {B, Tq, H, Dp}, type, on)), lse = saved_as(saved[5], {B, H, Tq}, at::kFloat, on).contiguous();
+            const Tensor lo = type == at::kFloat ? Tensor() : packed(saved_as(saved[4], {B, Tq, H, Dp}, type, on));
+            const auto lens = [&](const Tensor& t) { return t.defined() ? saved_as(t, {B}, at::kInt, on).contiguous() : Tensor(); };
+            const Tensor ql = lens(saved[6]), kl = lens(saved[7]);
             Tensor d[3] = {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(k.sizes(), k.options())};
             if (q.numel() == 0 || k.numel() == 0) {
                 for (auto& t : d) t.zero_();
             } else {
-                PpvAttention a = describe(q, k, v, out, saved[4], saved[5], saved[6], saved[7], ctx->saved_data["causal"].toBool(),
-                                          ctx->saved_data["scale"].toDouble());
-                const Tensor g = operand(grads[0], out.size(3));
+                PpvAttention a = describe(q, k, v, out, lo, lse, ql, kl, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+                const Tensor g = operand(go, Dp);
                 a.dout = g.data_ptr();
                 a.sgb = stride_of(g, 0); a.sgt = stride_of(g, 1); a.sgh = stride_of(g, 2);
                 a.dq = d[0].data_ptr(); a.dk = d[1].data_ptr(); a.dv = d[2].data_ptr();

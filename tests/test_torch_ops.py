@@ -150,3 +150,42 @@ def test_builds_of_one_torch_release_are_one(version, monkeypatch):
     monkeypatch.setattr(torch, "__version__", mod.torch_version + "7" + version)
     with pytest.raises(RuntimeError, match="stale build"):
         _lib._check_torch_ops(mod)
+
+
+def _train_step(norm, attend, x, w, q, k, v, lens):
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, q, k, v)]
+    y = norm(leaves[0], leaves[1])
+    o = attend(*leaves[2:], causal=True, q_lens=lens, k_lens=lens)
+    return (y.detach(), o.detach()) + torch.autograd.grad((y, o), leaves, (torch.cos(y.detach()), torch.cos(o.detach())))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_saved_tensors_may_go_away_and_come_back(dt):
+    """Through host memory, in another order of memory, at another alignment: the same bits.  What comes back on another device, in another size or type is an
+    error, never an address for a kernel."""
+    norm, attend = _public()
+    gen = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=gen).cuda().to(dt)
+    args = (r(7, 40), r(40), r(3, 9, 4, 20), r(3, 11, 2, 20), r(3, 11, 2, 20), torch.tensor([9, 4, 0], dtype=torch.int32, device="cuda"))
+    want = _train_step(norm, attend, *args)
+
+    def backwards(t):                                           # the same values, memory in the reversed order of axes
+        return t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))
+
+    def off(t):                                                 # one element behind a multiple of 16 bytes
+        f = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return f.copy_(t)
+
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    for ctx in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True), hooks(backwards, lambda t: t), hooks(off, lambda t: t)):
+        with ctx:
+            got = _train_step(norm, attend, *args)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for wrong in (lambda t: t.cpu(), lambda t: t.double() if t.is_floating_point() else t.long(), lambda t: t[:-1], lambda t: t[None]):
+        for call, leaf in ((lambda a: norm(a, args[1]), args[0]), (lambda a: attend(a, args[3], args[4], q_lens=args[5]), args[2])):
+            a = leaf.clone().requires_grad_(True)
+            with hooks(wrong, lambda t: t):
+                y = call(a)
+            with pytest.raises(RuntimeError, match="came back from its hooks"):
+                y.sum().backward()
